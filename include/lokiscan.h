@@ -42,7 +42,8 @@ typedef enum {
 typedef enum {
     LK_F32 = 0, /* L2-normalised float32: the reference's own representation */
     LK_F16 = 1, /* L2-normalised, rounded to IEEE half */
-    LK_I8 = 2   /* L2-normalised, per-row symmetric int8 codes + float32 scale */
+    LK_I8 = 2,  /* L2-normalised, per-row symmetric int8 codes + float32 scale */
+    LK_BF16 = 3 /* bfloat16: element type of the operators on device tensors, not a storage type */
 } lk_dtype;
 
 /* Scoring mode of a query: media-server/embedindex/embedindex.go:64-77. */
@@ -326,6 +327,87 @@ LK_API int lk_seed_scores(const float *cands, int64_t n_cand, const float *seeds
  *             to the reference's for that count.  The variance fractions agree to ~1e-13
  *             relative (the reference sums the total variance as one long chain). */
 LK_API int lk_pca3(const float *vecs, int64_t n, int dim, int workers, int device, float *coords, double *variance);
+
+/* ---- operators on device tensors (no counterpart in the reference) --------- */
+
+/* From a model's hidden states to rows and answers: the norm that turns hidden states into int8
+ * rows with scales, the matrix product that reads such rows (or 16-bit ones), and the draw among
+ * scored rows.  All pointers but the handles are DEVICE pointers on `device`, owned by the caller;
+ * the calls allocate nothing, need no workspace, enqueue on `stream` (a cudaStream_t, NULL = default
+ * stream) and return without waiting, so they can be captured into a graph and overlap freely with
+ * each other.  The caller's current device is the same after the call as before it.  Strides (ld*)
+ * are in ELEMENTS between the starts of consecutive rows; the elements of a row are contiguous.
+ * Nothing outside the stated rows and columns is read or written.  Outputs must not overlap inputs
+ * except where said.  A size of zero rows (or columns) is a call that does nothing. */
+
+/* Root-mean-square norm of x (+ residual) to 8 bits, row by row:
+ *   h = x + residual (float32);  y = h / sqrt(mean(h^2) + eps) * gain;
+ *   scale = max|y| / 127;  code = round(y / scale), half to even, in [-127, 127]
+ * i.e. the row format of LK_I8 (with unit gain and eps = 0: the codes of the L2-normalised row, its
+ * scale times sqrt(dim)).  The norm is taken of h before it is rounded to the type of `d_sum`.
+ *   dtype       LK_F32 / LK_F16 / LK_BF16: type of x, residual and sum
+ *   dim         1..LK_NORM_MAX_DIM
+ *   d_residual  NULL = none
+ *   d_gain      NULL = ones; else dim values of gain_dtype (LK_F32 / LK_F16 / LK_BF16)
+ *   d_sum       NULL, or h rounded to dtype (the residual of the next layer); may be the same
+ *               array as d_x or d_residual, with the same stride
+ *   d_codes     rows x dim int8;  d_scales rows floats
+ * A row of zeros gets scale 0 and codes 0; a row in which h or y has a NaN or an infinity gets
+ * scale NaN and codes 0, so that whatever is computed from it is NaN. */
+#define LK_NORM_MAX_DIM 32768
+LK_API int lk_rms_norm_i8(int device, int dtype, int64_t rows, int dim, const void *d_x, int64_t ldx,
+                          const void *d_residual, int64_t ldr, const void *d_gain, int gain_dtype, float eps,
+                          void *d_sum, int64_t lds, int8_t *d_codes, int64_t ldc, float *d_scales, void *stream);
+
+/* Matrix product of rows with rows, with its epilogue:
+ *   out[i, j] = act(scale_a[i] * scale_w[j] * sum_l a[i, l] * w[j, l] + bias[j]) + residual[i, j]
+ * rounded once, to out_dtype.  For LK_I8 the sum is the exact int32 dot (as in lk_search); for
+ * LK_F16 / LK_BF16 products are exact and accumulated in float32.
+ *   dtype       LK_I8, LK_F16 or LK_BF16: type of a (m x k) and w (n x k)
+ *   k           at most LK_LINEAR_MAX_K; k = 0 gives act(bias) + residual
+ *   d_a_scales  m floats, d_w_scales n floats; each may be NULL (ones)
+ *   d_bias      NULL, or n values of out_dtype
+ *   act         lk_act
+ *   d_residual  NULL, or m x n of out_dtype; may be d_out itself, with the same stride
+ *   d_out       m x n of out_dtype: LK_F32, LK_F16 or LK_BF16
+ * Rows of a and w that start on 16-byte boundaries (base and stride) take the tensor cores; others
+ * are computed by a slower kernel. */
+typedef enum {
+    LK_ACT_NONE = 0,
+    LK_ACT_RELU = 1,
+    LK_ACT_SILU = 2,     /* v / (1 + exp(-v)) */
+    LK_ACT_GELU = 3,     /* v * (1 + erf(v / sqrt 2)) / 2 */
+    LK_ACT_GELU_TANH = 4 /* v * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) / 2 */
+} lk_act;
+#define LK_LINEAR_MAX_K 65536
+LK_API int lk_linear(int device, int dtype, int64_t m, int64_t n, int64_t k, const void *d_a, int64_t lda,
+                     const float *d_a_scales, const void *d_w, int64_t ldw, const float *d_w_scales,
+                     const void *d_bias, int act, const void *d_residual, int64_t ldr,
+                     int out_dtype, void *d_out, int64_t ldo, void *stream);
+
+/* One draw per row of scores, from given random numbers.  Order of a row: score descending, index
+ * ascending on equal scores (as in lk_search; -0 equals +0).  Weights w = exp((x - max x) / T); kept is
+ * a prefix of the order: the top_k first; of those the shortest prefix that holds top_p of their
+ * weight (at least one); of those the ones with w >= min_p (at least the first).  The draw is the
+ * first INDEX (ascending) at which the running sum of the kept weights exceeds u times their sum.
+ * Weights are summed as 64-bit integers (fixed point), so the result does not depend on an order
+ * of additions: the same inputs give the same draw on every call.
+ *   dtype          LK_F32 / LK_F16 / LK_BF16: type of the rows x vocab scores
+ *   vocab          at most LK_SAMPLE_MAX_VOCAB
+ *   d_temperature  rows floats, NULL = 1 everywhere; 0 = the largest score (top_k = 1)
+ *   d_top_k        rows int32, NULL or <= 0 = all
+ *   d_top_p        rows floats, NULL or >= 1 = all; <= 0 = only the first
+ *   d_min_p        rows floats, NULL or <= 0 = all
+ *   d_u            rows floats in [0, 1); others are taken as the nearest number of that range
+ *   d_ids          rows int64;  d_probs (may be NULL) the weight of the draw over the kept weight;
+ *                  d_kept (may be NULL) how many were kept
+ * NaN and -infinity are never drawn; +infinity takes all weight (shared where there are several).
+ * A row with nothing to draw, or whose temperature is negative or NaN, or whose top_p, min_p or u
+ * is NaN, gets id -1, probability 0, kept 0. */
+#define LK_SAMPLE_MAX_VOCAB 16777216
+LK_API int lk_sample(int device, int dtype, int64_t rows, int64_t vocab, const void *d_logits, int64_t ld,
+                     const float *d_temperature, const int32_t *d_top_k, const float *d_top_p, const float *d_min_p,
+                     const float *d_u, int64_t *d_ids, float *d_probs, int32_t *d_kept, void *stream);
 
 /* ---- statistics ----------------------------------------------------------- */
 

@@ -20,7 +20,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "liblokiscan.so")
 
 LK_OK, LK_EINVAL, LK_EDIM, LK_ENOMEM, LK_ECUDA, LK_ENCCL, LK_ETIMEOUT, LK_ERANGE = range(8)
-LK_F32, LK_F16, LK_I8 = 0, 1, 2
+LK_F32, LK_F16, LK_I8, LK_BF16 = 0, 1, 2, 3
 LK_SCORE_DEFAULT, LK_SCORE_PLAIN = 0, 1
 LK_MIN_CENTER_COUNT = 64
 
@@ -102,6 +102,9 @@ _sig("lk_prescreen_pairs", _int, _vp, _i64, _int, C.c_float, _int, _vp, _vp, _vp
 _sig("lk_pca3", _int, _vp, _i64, _int, _int, _int, _vp, _vp)
 _sig("lk_seed_scores", _int, _vp, _i64, _vp, _i64, _int, C.c_float, _i64, _int, _vp, _vp, _vp, _i64, _vp)
 _sig("lk_scan_i8_prealloc", _int, _int, _vp, _i64, _int, _i64, _vp, _vp, C.c_float, _int, _vp, _vp, _vp, _vp, _vp)
+_sig("lk_rms_norm_i8", _int, _int, _int, _i64, _int, _vp, _i64, _vp, _i64, _vp, _int, C.c_float, _vp, _i64, _vp, _i64, _vp, _vp)
+_sig("lk_linear", _int, _int, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _vp, _i64, _int, _vp, _i64, _vp)
+_sig("lk_sample", _int, _int, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp)
 LK_PREALLOC_MAX_K = 128
 
 
