@@ -385,6 +385,11 @@ LK_API int lk_linear(int device, int dtype, int64_t m, int64_t n, int64_t k, con
                      const void *d_bias, int act, const void *d_residual, int64_t ldr,
                      int out_dtype, void *d_out, int64_t ldo, void *stream);
 
+/* Waits for the device and reports whether a bounded wait inside a kernel of these operators ran out
+ * since the last such call: LK_ETIMEOUT if so (results of calls since then may be incomplete).  A copy
+ * that does not arrive within 2 s is the only cause.  Not for use during a stream capture. */
+LK_API int lk_ops_status(int device);
+
 /* One draw per row of scores, from given random numbers.  Order of a row: score descending, index
  * ascending on equal scores (as in lk_search; -0 equals +0).  Weights w = exp((x - max x) / T); kept is
  * a prefix of the order: the top_k first; of those the shortest prefix that holds top_p of their

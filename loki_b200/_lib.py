@@ -104,6 +104,7 @@ _sig("lk_seed_scores", _int, _vp, _i64, _vp, _i64, _int, C.c_float, _i64, _int, 
 _sig("lk_scan_i8_prealloc", _int, _int, _vp, _i64, _int, _i64, _vp, _vp, C.c_float, _int, _vp, _vp, _vp, _vp, _vp)
 _sig("lk_rms_norm_i8", _int, _int, _int, _i64, _int, _vp, _i64, _vp, _i64, _vp, _int, C.c_float, _vp, _i64, _vp, _i64, _vp, _vp)
 _sig("lk_linear", _int, _int, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _vp, _i64, _int, _vp, _i64, _vp)
+_sig("lk_ops_status", _int, _int)
 _sig("lk_sample", _int, _int, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp)
 LK_PREALLOC_MAX_K = 128
 

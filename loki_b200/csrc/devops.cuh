@@ -98,6 +98,13 @@ class DeviceScope {
     int prev_ = -1;
 };
 
+// SMs of a device, asked once.
+inline int sm_count(int device) {
+    static int known[kMaxDevices];
+    if (known[device] == 0 && cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess) known[device] = 148;
+    return known[device];
+}
+
 // Launches through the call that returns this launch's own error: nothing another library left pending is
 // taken for it.
 template <typename... P, typename... A>

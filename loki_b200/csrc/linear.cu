@@ -5,8 +5,6 @@
 // 32 columns at a time with one load per element.  int8 sums are exact in int32, 16-bit ones accumulate in
 // float32 in the order of k.  Bound: the FMA pipes and its scalar loads; it exists for rows that do not
 // start on 16-byte boundaries, which the tensor-core kernels' copies cannot read.
-#include <cfloat>
-
 #include "linear.cuh"
 
 namespace lk {
@@ -95,7 +93,16 @@ extern "C" int lk_linear(int device, int dtype, int64_t m, int64_t n, int64_t k,
     if (!some) return LK_OK;
     const LinearArgs p = {d_a, d_w, d_a_scales, d_w_scales, d_bias, d_residual, d_out, m, n, k, lda, ldw, ldr, ldo, act, out_dtype};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (linear_mma_reads(p, dtype)) return linear_mma_launch(p, dtype, device, st);
     if (dtype == LK_I8) return any_launch<signed char>(p, st);
     if (dtype == LK_F16) return any_launch<__half>(p, st);
     return any_launch<__nv_bfloat16>(p, st);
+}
+
+extern "C" int lk_ops_status(int device) {
+    DeviceScope scope;
+    LK_TRY(scope.enter(device, "lk_ops_status"));
+    int failed = 0;
+    LK_TRY(linear_failed(&failed));
+    return failed ? fail(LK_ETIMEOUT, "lk_linear: a bounded wait inside the kernel ran out; its results are not complete") : LK_OK;
 }

@@ -14,17 +14,25 @@ struct LinearArgs {
     int act, out_type;
 };
 
-__device__ __forceinline__ float activate(int act, float v) {
-    switch (act) {
-        case LK_ACT_RELU: return v < 0.0f ? 0.0f : v;  // NaN stays
-        case LK_ACT_SILU: return v / (1.0f + __expf(-v));
-        case LK_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-        case LK_ACT_GELU_TANH: {
-            // (1 + tanh z) / 2 = 1 / (1 + exp(-2 z))
-            const float z = 0.79788456080286536f * (v + 0.044715f * v * v * v);
-            return v / (1.0f + __expf(-2.0f * z));
+// The activation of N values: one branch for all of them.
+template <int N>
+__device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
+    if (act == LK_ACT_RELU) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] = v[u] < 0.0f ? 0.0f : v[u];  // NaN stays
+    } else if (act == LK_ACT_SILU) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] = v[u] / (1.0f + __expf(-v[u]));
+    } else if (act == LK_ACT_GELU) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] = 0.5f * v[u] * (1.0f + erff(v[u] * 0.70710678118654752f));
+    } else if (act == LK_ACT_GELU_TANH) {
+        // (1 + tanh z) / 2 = 1 / (1 + exp(-2 z))
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const float z = 0.79788456080286536f * (v[u] + 0.044715f * v[u] * v[u] * v[u]);
+            v[u] = v[u] / (1.0f + __expf(-2.0f * z));
         }
-        default: return v;
     }
 }
 
@@ -40,9 +48,16 @@ __device__ __forceinline__ void store_as(int dtype, void *p, long long i, float 
 __device__ __forceinline__ void finish_one(const LinearArgs &p, long long i, long long j, float acc) {
     float v = acc * (scale_of(p.a_scales, i) * scale_of(p.w_scales, j));
     if (p.bias != nullptr) v += load_as(p.out_type, p.bias, j);
-    v = activate(p.act, v);
-    if (p.residual != nullptr) v += load_as(p.out_type, p.residual, i * p.ldr + j);
-    store_as(p.out_type, p.out, i * p.ldo + j, v);
+    float y[1] = {v};
+    activate_all<1>(p.act, y);
+    if (p.residual != nullptr) y[0] += load_as(p.out_type, p.residual, i * p.ldr + j);
+    store_as(p.out_type, p.out, i * p.ldo + j, y[0]);
 }
+
+// linear_mma.cu: whether the tensor-core kernel's copies can read these operands, and its launch.
+bool linear_mma_reads(const LinearArgs &p, int dtype);
+int linear_mma_launch(const LinearArgs &p, int dtype, int device, cudaStream_t st);
+// Whether one of its bounded waits ran out on the current device since the last call; waits for the device.
+int linear_failed(int *out);
 
 }  // namespace lk

@@ -1,0 +1,406 @@
+// Matrix product of rows with rows on the tensor cores (tcgen05.mma, accumulators in tensor memory), the
+// scales, bias, activation and residual in its epilogue.
+//
+// The rows of w take the M side of the MMA (tensor-memory lanes), the rows of a its N side (columns): a
+// tile is 128 rows of w per CTA and `mt` rows of a, mt from 16 (single tokens: the MMA's smallest N) to 256.
+// One kernel thus serves one token and thousands, and an epilogue thread owns one column j of the
+// result: its scale and bias are two registers, and the 32 threads of a warp read the residual and write
+// the result 32 neighbours at a time, with no staging.
+//
+// Both operands arrive as [rows x 128 bytes] slices of K by TMA (128-byte swizzle), rows and columns past
+// the ends as zeros, through a ring of stages; 128 bytes are 128 int8 or 64 16-bit elements, four
+// MMAs either way.  Roles of a CTA: warp 0 issues the copies, warp 1 the MMAs, warps 2-9 are the epilogue (two
+// accumulators: a tile's epilogue runs under the next tile's MMAs).
+//
+// Two forms.  PAIR: two CTAs of a cluster share every MMA (cta_group::2, 256 rows of w), each loads its
+// own 128 rows of w and half the rows of a.  Single: one CTA per tile, and where there are too few tiles
+// to fill the GPU a cluster of `split` CTAs shares one tile's K: each sums its part, the parts are
+// exchanged through distributed shared memory, added in rank order (the result does not depend on timing),
+// and every CTA finishes its share of the columns.  No workspace, no atomics.
+//
+// Every wait is bounded; a CTA that gives up raises g_linear_failed, which lk_ops_status reports.
+#include "linear.cuh"
+#include "tensor5.cuh"
+
+namespace lk {
+
+constexpr int LW = 128;             // rows of w per CTA (tensor-memory lanes)
+constexpr int LSLICE = 128;         // bytes of K per stage: one swizzle row
+constexpr int LW_BYTES = LW * LSLICE;
+constexpr int LEPI_WARPS = 8;
+constexpr int LTHREADS = 64 + LEPI_WARPS * 32;
+constexpr int LMAX_STAGES = 12;
+constexpr int LCHUNK = 16;          // columns an epilogue thread holds at a time
+
+static __device__ unsigned g_linear_failed;  // a bounded wait ran out on this device
+
+struct LinearTiles {
+    int mt;              // rows of a per tile
+    int stages, split;
+    int slices;          // K slices of 128 bytes
+    int tiles_m;
+    long long tiles;
+    unsigned idesc;
+    unsigned columns;    // tensor memory to allocate
+};
+
+struct LinearShared {
+    unsigned long long full[LMAX_STAGES], empty[LMAX_STAGES], acc_full[2], acc_empty[2];
+    unsigned tmem_base;
+    int failed;
+};
+
+// 2-D tiled TMA load into this CTA's shared memory, counted on `bar` (PAIR: the leader's).
+template <bool PAIR>
+__device__ __forceinline__ void l_load(unsigned dst, const CUtensorMap *tm, int x, int y, unsigned bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(reinterpret_cast<unsigned long long>(tm)), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(reinterpret_cast<unsigned long long>(tm)), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+
+template <bool PAIR, bool I8>
+__device__ __forceinline__ void l_mma(unsigned d, unsigned long long dw, unsigned long long da, unsigned idesc, bool accumulate) {
+    const unsigned acc = accumulate ? 1u : 0u;
+#define LK_MMA(GROUP, KIND)                                                              \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                       \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}" \
+                 ::"r"(d), "l"(dw), "l"(da), "r"(idesc), "r"(acc) : "memory")
+    if constexpr (PAIR && I8) LK_MMA("2", "i8");
+    else if constexpr (PAIR) LK_MMA("2", "f16");
+    else if constexpr (I8) LK_MMA("1", "i8");
+    else LK_MMA("1", "f16");
+#undef LK_MMA
+}
+
+// Arrive on `bar` (PAIR: at its address in both CTAs) once the MMAs issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void l_commit(unsigned long long *bar) {
+    if constexpr (PAIR) g_mma_commit(bar);
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(g_smem(bar)) : "memory");
+}
+
+__device__ __forceinline__ void l_tmem_ld16(unsigned taddr, unsigned (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+template <bool I8>
+__device__ __forceinline__ float l_sum(unsigned bits) {
+    if constexpr (I8) return (float)(int)bits;
+    else return __uint_as_float(bits);
+}
+
+template <bool PAIR, bool I8, typename Out>
+__global__ void __launch_bounds__(LTHREADS, 1)
+k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const LinearArgs p, const LinearTiles g) {
+    constexpr int CG = PAIR ? 2 : 1;
+    extern __shared__ unsigned char l_raw[];
+    // 1024-byte alignment: the swizzle pattern is a function of the shared-memory address
+    unsigned char *smem = l_raw + ((1024u - (g_smem(l_raw) & 1023u)) & 1023u);
+    const int a_bytes = g.mt / CG * LSLICE;
+    unsigned char *sm_w = smem;                                    // [stages][128 rows][128 B]
+    unsigned char *sm_a = sm_w + (size_t)g.stages * LW_BYTES;      // [stages][mt / CG rows][128 B]
+    LinearShared *ctl = reinterpret_cast<LinearShared *>(sm_a + (size_t)g.stages * a_bytes);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = PAIR || g.split > 1 ? (int)g_cta_rank() : 0;
+    const int cta_of = PAIR ? rank : 0;          // which half of the pair's tile
+    const int part_of = PAIR ? 0 : rank;         // which part of K
+    const int per = PAIR ? 2 : g.split;          // CTAs per tile
+    const long long first = blockIdx.x / per, step = gridDim.x / per;
+    const int s0 = (int)((long long)g.slices * part_of / (PAIR ? 1 : g.split));
+    const int s1 = (int)((long long)g.slices * (part_of + 1) / (PAIR ? 1 : g.split));
+
+    if (tid == 0) {
+        for (int i = 0; i < g.stages; ++i) {
+            g_mbar_init(&ctl->full[i], 1);
+            g_mbar_init(&ctl->empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            g_mbar_init(&ctl->acc_full[i], 1);
+            g_mbar_init(&ctl->acc_empty[i], CG * LEPI_WARPS);
+        }
+        ctl->failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        __syncwarp();
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(g_smem(&ctl->tmem_base)), "r"(g.columns) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(g_smem(&ctl->tmem_base)), "r"(g.columns) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (PAIR) g_pair_sync();  // the partner's barriers exist before anything is signalled across
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = ctl->tmem_base;
+    volatile int *failed = &ctl->failed;
+
+    if (warp == 0) {
+        // ------------------------------ copies ------------------------------
+        int stage = 0;
+        unsigned phase = 0;
+        bool ok = true;
+        for (long long t = first; ok && t < g.tiles; t += step) {
+            const int yw = (int)(t / g.tiles_m) * LW * CG + cta_of * LW;
+            const int ya = (int)(t % g.tiles_m) * g.mt + cta_of * (g.mt / CG);
+            for (int s = s0; s < s1; ++s) {
+                ok = g_mbar_wait_warp(&ctl->empty[stage], phase ^ 1u, failed);
+                if (!ok) break;
+                if (g_elect_one()) {
+                    const unsigned bar = PAIR ? g_leader_addr(g_smem(&ctl->full[stage])) : g_smem(&ctl->full[stage]);
+                    if (cta_of == 0) g_mbar_expect_tx(&ctl->full[stage], (unsigned)(CG * (LW_BYTES + a_bytes)));
+                    l_load<PAIR>(g_smem(sm_w + (size_t)stage * LW_BYTES), &tm_w, s * LSLICE, yw, bar);
+                    l_load<PAIR>(g_smem(sm_a + (size_t)stage * a_bytes), &tm_a, s * LSLICE, ya, bar);
+                }
+                __syncwarp();
+                if (++stage == g.stages) stage = 0, phase ^= 1u;
+            }
+        }
+    } else if (warp == 1 && cta_of == 0) {
+        // ------------------------------ MMAs ------------------------------
+        const unsigned long long dw0 = g_smem_desc(g_smem(sm_w)), da0 = g_smem_desc(g_smem(sm_a));
+        int stage = 0, acc = 0;
+        unsigned phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (long long t = first; ok && t < g.tiles; t += step) {
+            ok = g_mbar_wait_warp(&ctl->acc_empty[acc], acc_phase ^ 1u, failed);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const unsigned d = tmem + (unsigned)(acc * g.mt);
+            for (int s = s0; s < s1; ++s) {
+                ok = g_mbar_wait_warp(&ctl->full[stage], phase, failed);
+                if (!ok) break;
+                // the start-address field counts 16-byte units
+                const unsigned long long dw = dw0 + (unsigned long long)(stage * (LW_BYTES >> 4));
+                const unsigned long long da = da0 + (unsigned long long)(stage * (a_bytes >> 4));
+                if (g_elect_one()) {
+#pragma unroll
+                    for (int q = 0; q < LSLICE / 32; ++q)  // 32 bytes of K per MMA
+                        l_mma<PAIR, I8>(d, dw + (unsigned long long)(2 * q), da + (unsigned long long)(2 * q), g.idesc, s != s0 || q != 0);
+                    l_commit<PAIR>(&ctl->empty[stage]);
+                }
+                __syncwarp();
+                if (++stage == g.stages) stage = 0, phase ^= 1u;
+            }
+            if (!ok) break;
+            if (g_elect_one()) l_commit<PAIR>(&ctl->acc_full[acc]);
+            __syncwarp();
+            if (++acc == 2) acc = 0, acc_phase ^= 1u;
+        }
+    } else if (warp >= 2) {
+        // ------------------------------ epilogue ------------------------------
+        const int quad = warp & 3, half = (warp - 2) >> 2;  // the lanes a warp may read; the chunks it takes
+        const Out *residual = static_cast<const Out *>(p.residual);
+        Out *out = static_cast<Out *>(p.out);
+        int acc = 0;
+        unsigned acc_phase = 0;
+        for (long long t = first; t < g.tiles; t += step) {
+            const long long j = (t / g.tiles_m) * (LW * CG) + cta_of * LW + quad * 32 + lane;
+            const long long i0 = (t % g.tiles_m) * g.mt;
+            const bool live = j < p.n;
+            const float sw = live ? scale_of(p.w_scales, j) : 0.0f;
+            const float bias = live && p.bias != nullptr ? Elem<Out>::get(static_cast<const Out *>(p.bias)[j]) : 0.0f;
+            if (!g_mbar_wait_warp(&ctl->acc_full[acc], acc_phase, failed)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int c = half * LCHUNK; c < g.mt; c += 2 * LCHUNK) {
+                unsigned v[LCHUNK];
+                l_tmem_ld16(tmem + (unsigned)(acc * g.mt + c) + ((unsigned)(quad * 32) << 16), v);
+                if (!PAIR && g.split > 1) {  // this CTA's part of the sums, to where the cluster can read it
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    unsigned *red = reinterpret_cast<unsigned *>(smem);
+#pragma unroll
+                    for (int u = 0; u < LCHUNK; ++u) red[(c + u) * LW + quad * 32 + lane] = v[u];
+                    continue;
+                }
+                const long long i = i0 + c;
+                const int rows = (int)min((long long)LCHUNK, p.m - i);
+                float r[LCHUNK], x[LCHUNK];
+                if (p.residual != nullptr) {
+#pragma unroll
+                    for (int u = 0; u < LCHUNK; ++u) r[u] = live && u < rows ? Elem<Out>::get(residual[(i + u) * p.ldr + j]) : 0.0f;
+                }
+                const float sa = p.a_scales != nullptr && lane < rows ? p.a_scales[i + lane] : 1.0f;  // lanes past the chunk are not asked
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int u = 0; u < LCHUNK; ++u) x[u] = l_sum<I8>(v[u]) * (__shfl_sync(0xffffffffu, sa, u) * sw) + bias;
+                activate_all<LCHUNK>(p.act, x);
+                if (p.residual != nullptr) {
+#pragma unroll
+                    for (int u = 0; u < LCHUNK; ++u) x[u] += r[u];
+                }
+#pragma unroll
+                for (int u = 0; u < LCHUNK; ++u)
+                    if (live && u < rows) out[(i + u) * p.ldo + j] = Elem<Out>::put(x[u]);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR) g_mbar_arrive_leader(&ctl->acc_empty[acc]);
+                else g_mbar_arrive(&ctl->acc_empty[acc]);
+            }
+            if (++acc == 2) acc = 0, acc_phase ^= 1u;
+        }
+    }
+    // ------------------------------ joining the parts of K ------------------------------
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (!PAIR && g.split > 1) {  // one tile per cluster
+        g_pair_sync();
+        const long long j0 = (first / g.tiles_m) * LW, i0 = (first % g.tiles_m) * g.mt;
+        const int lo = g.mt * part_of / g.split, hi = g.mt * (part_of + 1) / g.split;
+        const unsigned base = g_smem(smem);
+        for (int e = lo * LW + tid; e < hi * LW; e += LTHREADS) {
+            const long long i = i0 + e / LW, j = j0 + e % LW;
+            if (i >= p.m || j >= p.n) continue;
+            float x;
+            int whole = 0;
+            float sum = 0.0f;
+            for (int r = 0; r < g.split; ++r) {
+                unsigned at, bits;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + (unsigned)e * 4u), "r"(r));
+                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(bits) : "r"(at) : "memory");
+                if constexpr (I8) whole += (int)bits;
+                else sum += __uint_as_float(bits);
+            }
+            x = I8 ? (float)whole : sum;
+            float y[1] = {x * (scale_of(p.a_scales, i) * scale_of(p.w_scales, j)) +
+                          (p.bias != nullptr ? Elem<Out>::get(static_cast<const Out *>(p.bias)[j]) : 0.0f)};
+            activate_all<1>(p.act, y);
+            if (p.residual != nullptr) y[0] += Elem<Out>::get(static_cast<const Out *>(p.residual)[i * p.ldr + j]);
+            static_cast<Out *>(p.out)[i * p.ldo + j] = Elem<Out>::put(y[0]);
+        }
+    }
+    if (tid == 0 && ctl->failed != 0) {
+        atomicExch(&g_linear_failed, 1u);
+        // copies this CTA issued may still be landing in its shared memory: give them time before it is released
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000ll) {}
+    }
+    if (PAIR || g.split > 1) g_pair_sync();  // nothing of the cluster is still aimed at, or reading, this CTA
+    if (warp == 1) {
+        __syncwarp();
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.columns) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.columns) : "memory");
+    }
+}
+
+bool linear_mma_reads(const LinearArgs &p, int dtype) {
+    const int eb = type_bytes(dtype);
+    const auto reads = [&](const void *base, long long rows, long long ld) {
+        return reinterpret_cast<uintptr_t>(base) % 16 == 0 && (rows == 1 || (ld * eb % 16 == 0 && ld * eb < (1ll << 40)));
+    };
+    return p.k > 0 && reads(p.a, p.m, p.lda) && reads(p.w, p.n, p.ldw);
+}
+
+struct LinearPlan {
+    bool pair;
+    int mt, split;
+};
+
+// The tile that finishes first by a simple account of one CTA's clocks: a slice of K costs its MMAs (2 mt
+// clocks, never under 128: 128 rows of w read from shared memory) or its bytes at 40 per clock and SM, whichever is
+// more; a tile's last epilogue, a launch and an exchange of parts come on top.
+static LinearPlan linear_plan(long long m, long long n, int slices, int sms) {
+    LinearPlan best = {false, 16, 1};
+    double least = 1e300;
+    const auto offer = [&](bool pair, int mt, int split) {
+        const long long cg = pair ? 2 : 1;
+        const long long tiles = ((m + mt - 1) / mt) * ((n + LW * cg - 1) / (LW * cg));
+        const long long ctas = tiles * cg * split;
+        if (split > 1 && (ctas > sms || split > slices)) return;
+        const double waves = (double)((ctas + sms - 1) / sms);
+        const double slice = std::max(std::max(2.0 * mt, 128.0), (LW_BYTES + mt / cg * LSLICE) / 40.0);
+        const double cost = waves * ((slices + split - 1) / split) * slice + 20.0 * mt / split + (split > 1 ? 1500.0 + 100.0 * split : 0.0);
+        if (cost < least) least = cost, best = {pair, mt, split};
+    };
+    for (int mt = 16; mt <= 256; mt *= 2) {
+        if (mt >= 2 * m && mt > 16) break;  // a smaller tile holds all rows
+        for (int split = 1; split <= 8; split *= 2) offer(false, mt, split);
+        if (mt >= 128) offer(true, mt, 1);
+    }
+    return best;
+}
+
+template <bool PAIR, bool I8, typename Out>
+static int mma_launch(const CUtensorMap &tw, const CUtensorMap &ta, const LinearArgs &p, const LinearTiles &g, int device, int sms, cudaStream_t st) {
+    constexpr int CG = PAIR ? 2 : 1;
+    static bool sized[kMaxDevices];
+    const size_t smem = (size_t)g.stages * (LW_BYTES + g.mt / CG * LSLICE) + sizeof(LinearShared) + 1024;
+    if (!sized[device]) {
+        LK_CUDA(cudaFuncSetAttribute((const void *)k_linear_mma<PAIR, I8, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        sized[device] = true;
+    }
+    const int per = PAIR ? 2 : g.split;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(std::min<long long>(g.tiles, std::max(1, sms / per)) * per));
+    cfg.blockDim = dim3(LTHREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)per;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = per > 1 ? 1 : 0;
+    return launch_cfg("lk_linear", k_linear_mma<PAIR, I8, Out>, cfg, tw, ta, p, g);
+}
+
+template <bool PAIR, bool I8>
+static int mma_out(const CUtensorMap &tw, const CUtensorMap &ta, const LinearArgs &p, const LinearTiles &g, int device, int sms, cudaStream_t st) {
+    if (p.out_type == LK_F32) return mma_launch<PAIR, I8, float>(tw, ta, p, g, device, sms, st);
+    if (p.out_type == LK_F16) return mma_launch<PAIR, I8, __half>(tw, ta, p, g, device, sms, st);
+    return mma_launch<PAIR, I8, __nv_bfloat16>(tw, ta, p, g, device, sms, st);
+}
+
+int linear_mma_launch(const LinearArgs &p, int dtype, int device, cudaStream_t st) {
+    const int eb = type_bytes(dtype), sms = sm_count(device);
+    LinearTiles g;
+    g.slices = (int)((p.k * eb + LSLICE - 1) / LSLICE);
+    const LinearPlan plan = linear_plan(p.m, p.n, g.slices, sms);
+    const int cg = plan.pair ? 2 : 1;
+    g.mt = plan.mt;
+    g.split = plan.split;
+    g.tiles_m = (int)((p.m + g.mt - 1) / g.mt);
+    g.tiles = g.tiles_m * ((p.n + LW * cg - 1) / (LW * cg));
+    const int stage_bytes = LW_BYTES + g.mt / cg * LSLICE;
+    g.stages = std::min((226 * 1024 - (int)sizeof(LinearShared) - 1024) / stage_bytes, LMAX_STAGES);
+    g.columns = std::max(32u, 2u * (unsigned)g.mt);
+    const unsigned kinds = dtype == LK_I8 ? (2u << 4) | (1u << 7) | (1u << 10)  // int8 x int8 -> int32
+                           : dtype == LK_BF16 ? (1u << 4) | (1u << 7) | (1u << 10) : (1u << 4);  // -> float32
+    g.idesc = kinds | ((unsigned)(g.mt >> 3) << 17) | ((unsigned)((LW * cg) >> 4) << 24);
+    CUtensorMap tw, ta;
+    const long long row = p.k * eb, single = (row + 15) / 16 * 16;
+    LK_TRY(encode_rows(&tw, p.w, p.n, row, p.n == 1 ? single : p.ldw * eb, LW));
+    LK_TRY(encode_rows(&ta, p.a, p.m, row, p.m == 1 ? single : p.lda * eb, g.mt / cg));
+    const bool i8 = dtype == LK_I8;
+    if (plan.pair) return i8 ? mma_out<true, true>(tw, ta, p, g, device, sms, st) : mma_out<true, false>(tw, ta, p, g, device, sms, st);
+    return i8 ? mma_out<false, true>(tw, ta, p, g, device, sms, st) : mma_out<false, false>(tw, ta, p, g, device, sms, st);
+}
+
+// Whether a wait ran out on the device since the last call; the flag is lowered.
+int linear_failed(int *out) {
+    unsigned v = 0, zero = 0;
+    LK_CUDA(cudaMemcpyFromSymbol(&v, g_linear_failed, sizeof v));
+    if (v) LK_CUDA(cudaMemcpyToSymbol(g_linear_failed, &zero, sizeof zero));
+    *out = v != 0;
+    return 0;
+}
+
+}  // namespace lk

@@ -155,6 +155,12 @@ def linear(a, w, *, a_scales=None, w_scales=None, bias=None, act: str = "none", 
     return out
 
 
+def check_device(device=0):
+    """Wait for the device; raise if a bounded wait inside one of these kernels ran out since the last call."""
+    index = torch.device("cuda", device).index if isinstance(device, int) else torch.device(device).index
+    check(lib.lk_ops_status(index))
+
+
 def _per_row(v, what, dtype, rows, device):
     """One value per row: a vector, or a number for all rows."""
     if v is None or isinstance(v, torch.Tensor):
