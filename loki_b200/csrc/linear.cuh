@@ -22,7 +22,7 @@ __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
         for (int u = 0; u < N; ++u) v[u] = v[u] < 0.0f ? 0.0f : v[u];  // NaN stays
     } else if (act == LK_ACT_SILU) {
 #pragma unroll
-        for (int u = 0; u < N; ++u) v[u] = v[u] / (1.0f + __expf(-v[u]));
+        for (int u = 0; u < N; ++u) v[u] = __fdividef(v[u], 1.0f + __expf(-v[u]));
     } else if (act == LK_ACT_GELU) {
 #pragma unroll
         for (int u = 0; u < N; ++u) v[u] = 0.5f * v[u] * (1.0f + erff(v[u] * 0.70710678118654752f));
@@ -31,7 +31,7 @@ __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const float z = 0.79788456080286536f * (v[u] + 0.044715f * v[u] * v[u] * v[u]);
-            v[u] = v[u] / (1.0f + __expf(-2.0f * z));
+            v[u] = __fdividef(v[u], 1.0f + __expf(-2.0f * z));
         }
     }
 }

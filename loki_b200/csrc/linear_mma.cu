@@ -9,7 +9,7 @@
 //
 // Both operands arrive as [rows x 128 bytes] slices of K by TMA (128-byte swizzle), rows and columns past
 // the ends as zeros, through a ring of stages; 128 bytes are 128 int8 or 64 16-bit elements, four
-// MMAs either way.  Roles of a CTA: warp 0 issues the copies, warp 1 the MMAs, warps 2-9 are the epilogue (two
+// MMAs either way.  Roles of a CTA: warp 0 issues the copies, warp 1 the MMAs, warps 2-17 are the epilogue (two
 // accumulators: a tile's epilogue runs under the next tile's MMAs).
 //
 // Two forms.  PAIR: two CTAs of a cluster share every MMA (cta_group::2, 256 rows of w), each loads its
@@ -27,7 +27,7 @@ namespace lk {
 constexpr int LW = 128;             // rows of w per CTA (tensor-memory lanes)
 constexpr int LSLICE = 128;         // bytes of K per stage: one swizzle row
 constexpr int LW_BYTES = LW * LSLICE;
-constexpr int LEPI_WARPS = 8;
+constexpr int LEPI_WARPS = 16;      // four per tensor-memory quadrant, 16 columns of a tile at a time each
 constexpr int LTHREADS = 64 + LEPI_WARPS * 32;
 constexpr int LMAX_STAGES = 12;
 constexpr int LCHUNK = 16;          // columns an epilogue thread holds at a time
@@ -46,6 +46,7 @@ struct LinearTiles {
 
 struct LinearShared {
     unsigned long long full[LMAX_STAGES], empty[LMAX_STAGES], acc_full[2], acc_empty[2];
+    float sa[2][256];  // the scales of a tile's rows of a, per accumulator
     unsigned tmem_base;
     int failed;
 };
@@ -206,48 +207,87 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
         }
     } else if (warp >= 2) {
         // ------------------------------ epilogue ------------------------------
-        const int quad = warp & 3, half = (warp - 2) >> 2;  // the lanes a warp may read; the chunks it takes
-        const Out *residual = static_cast<const Out *>(p.residual);
-        Out *out = static_cast<Out *>(p.out);
+        const int quad = warp & 3, part = (warp - 2) >> 2;  // the lanes a warp may read; the chunks it takes
+        const int et = tid - 64;
+        const long long ldr = p.ldr * (long long)sizeof(Out), ldo = p.ldo * (long long)sizeof(Out);
+        bool epi_ok = true;
+        const bool joined = !PAIR && g.split > 1;
         int acc = 0;
         unsigned acc_phase = 0;
         for (long long t = first; t < g.tiles; t += step) {
             const long long j = (t / g.tiles_m) * (LW * CG) + cta_of * LW + quad * 32 + lane;
             const long long i0 = (t % g.tiles_m) * g.mt;
             const bool live = j < p.n;
+            const bool whole = i0 + g.mt <= p.m && (j | 31) < p.n;  // this warp's share lies inside the result
             const float sw = live ? scale_of(p.w_scales, j) : 0.0f;
             const float bias = live && p.bias != nullptr ? Elem<Out>::get(static_cast<const Out *>(p.bias)[j]) : 0.0f;
-            if (!g_mbar_wait_warp(&ctl->acc_full[acc], acc_phase, failed)) break;
+            const char *res = static_cast<const char *>(p.residual) + i0 * ldr + j * (long long)sizeof(Out);
+            char *out = static_cast<char *>(p.out) + i0 * ldo + j * (long long)sizeof(Out);
+            // the residual of the chunk that comes next, fetched while the one before it is worked on (the first
+            // while the MMAs still run)
+            Out r[LCHUNK];
+            const auto fetch = [&](int c) {
+                const char *q = res + c * ldr;
+#pragma unroll
+                for (int u = 0; u < LCHUNK; ++u, q += ldr)
+                    if (whole || (live && i0 + c + u < p.m)) r[u] = *reinterpret_cast<const Out *>(q);
+            };
+            if (!joined) {
+                // the tile before last, which read this buffer, is behind every warp's last arrival at this barrier
+                if (p.a_scales != nullptr && et < g.mt) ctl->sa[acc][et] = i0 + et < p.m ? p.a_scales[i0 + et] : 0.0f;
+                if (p.residual != nullptr && part * LCHUNK < g.mt) fetch(part * LCHUNK);
+                asm volatile("bar.sync 1, %0;" ::"n"(LEPI_WARPS * 32) : "memory");
+            }
+            if (!g_mbar_wait_warp(&ctl->acc_full[acc], acc_phase, failed)) epi_ok = false;
+            if (!epi_ok) {
+                // the other warps of the epilogue may be waiting at the barrier above: stay with them to the last tile
+                if (++acc == 2) acc = 0, acc_phase ^= 1u;
+                continue;
+            }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int c = half * LCHUNK; c < g.mt; c += 2 * LCHUNK) {
+            for (int c = part * LCHUNK; c < g.mt; c += 4 * LCHUNK) {
                 unsigned v[LCHUNK];
                 l_tmem_ld16(tmem + (unsigned)(acc * g.mt + c) + ((unsigned)(quad * 32) << 16), v);
-                if (!PAIR && g.split > 1) {  // this CTA's part of the sums, to where the cluster can read it
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    unsigned *red = reinterpret_cast<unsigned *>(smem);
+                float rx[LCHUNK], x[LCHUNK];
+                if (p.residual != nullptr && !joined) {
 #pragma unroll
-                    for (int u = 0; u < LCHUNK; ++u) red[(c + u) * LW + quad * 32 + lane] = v[u];
+                    for (int u = 0; u < LCHUNK; ++u) rx[u] = Elem<Out>::get(r[u]);
+                    if (c + 4 * LCHUNK < g.mt) fetch(c + 4 * LCHUNK);
+                }
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (joined) {  // this CTA's part of the sums, to where the cluster can read it
+                    unsigned *red = reinterpret_cast<unsigned *>(smem) + c * LW + quad * 32 + lane;
+#pragma unroll
+                    for (int u = 0; u < LCHUNK; ++u) red[u * LW] = v[u];
                     continue;
                 }
-                const long long i = i0 + c;
-                const int rows = (int)min((long long)LCHUNK, p.m - i);
-                float r[LCHUNK], x[LCHUNK];
-                if (p.residual != nullptr) {
+                if (p.a_scales != nullptr) {
 #pragma unroll
-                    for (int u = 0; u < LCHUNK; ++u) r[u] = live && u < rows ? Elem<Out>::get(residual[(i + u) * p.ldr + j]) : 0.0f;
+                    for (int u = 0; u < LCHUNK; u += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(&ctl->sa[acc][c + u]);
+                        x[u] = fmaf(l_sum<I8>(v[u]), f.x * sw, bias);
+                        x[u + 1] = fmaf(l_sum<I8>(v[u + 1]), f.y * sw, bias);
+                        x[u + 2] = fmaf(l_sum<I8>(v[u + 2]), f.z * sw, bias);
+                        x[u + 3] = fmaf(l_sum<I8>(v[u + 3]), f.w * sw, bias);
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < LCHUNK; ++u) x[u] = fmaf(l_sum<I8>(v[u]), sw, bias);
                 }
-                const float sa = p.a_scales != nullptr && lane < rows ? p.a_scales[i + lane] : 1.0f;  // lanes past the chunk are not asked
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                for (int u = 0; u < LCHUNK; ++u) x[u] = l_sum<I8>(v[u]) * (__shfl_sync(0xffffffffu, sa, u) * sw) + bias;
                 activate_all<LCHUNK>(p.act, x);
                 if (p.residual != nullptr) {
 #pragma unroll
-                    for (int u = 0; u < LCHUNK; ++u) x[u] += r[u];
+                    for (int u = 0; u < LCHUNK; ++u) x[u] += rx[u];
                 }
+                char *q = out + c * ldo;
+                if (whole) {
 #pragma unroll
-                for (int u = 0; u < LCHUNK; ++u)
-                    if (live && u < rows) out[(i + u) * p.ldo + j] = Elem<Out>::put(x[u]);
+                    for (int u = 0; u < LCHUNK; ++u, q += ldo) *reinterpret_cast<Out *>(q) = Elem<Out>::put(x[u]);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < LCHUNK; ++u, q += ldo)
+                        if (live && i0 + c + u < p.m) *reinterpret_cast<Out *>(q) = Elem<Out>::put(x[u]);
+                }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
