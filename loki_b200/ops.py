@@ -30,51 +30,63 @@ def _refuse(status, message):
     raise LokiError(status, message)
 
 
-def _ready(t, what, types, device=None, dims=2):
-    """A tensor that the kernels can read: its type, its device, contiguous rows, no gradient."""
+def _why(t, what, types, index, *shape):
+    """The refusal of a tensor that :func:`_matrix` or :func:`_vector` found wrong."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _refuse(LK_EINVAL, f"{what}: a CUDA tensor is wanted (this library has no CPU path)")
     if t.dtype not in types:
         _refuse(LK_EINVAL, f"{what}: {t.dtype} is not supported here")
-    if t.dim() != dims:
-        _refuse(LK_EDIM, f"{what}: {dims} dimension(s) are wanted, not {t.dim()}")
+    if t.dim() != len(shape):
+        _refuse(LK_EDIM, f"{what}: {len(shape)} dimension(s) are wanted, not {t.dim()}")
+    if index is not None and t.get_device() != index:
+        _refuse(LK_EINVAL, f"{what}: it is on {t.device}, not on cuda:{index}")
+    if any(want is not None and have != want for have, want in zip(t.shape, shape)):
+        _refuse(LK_EDIM, f"{what}: shape {tuple(t.shape)} where {shape} is wanted")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         _refuse(LK_EINVAL, f"{what}: its rows are not contiguous")
-    if dims == 2 and t.shape[0] > 1 and t.shape[1] > 0 and t.stride(0) < t.shape[1]:
-        _refuse(LK_EINVAL, f"{what}: its rows overlap")
-    if device is not None and t.device != device:
-        _refuse(LK_EINVAL, f"{what}: it is on {t.device}, not on {device}")
     if t.requires_grad and torch.is_grad_enabled():
         _refuse(LK_EINVAL, f"{what}: it requires a gradient, which this operator does not have")
-    return t
+    _refuse(LK_EINVAL, f"{what}: its rows overlap")
 
 
-def _shaped(t, what, types, device, *shape):
-    _ready(t, what, types, device, len(shape))
-    if tuple(t.shape) != shape:
-        _refuse(LK_EDIM, f"{what}: shape {tuple(t.shape)} where {shape} is wanted")
-    return t
+# The two checks below run on every call: they ask a tensor for as little as possible.
+
+def _matrix(t, what, types, index=None, rows=None, cols=None):
+    """(rows, cols, elements between rows, device) of a matrix that the kernels can read."""
+    try:
+        on = t.get_device()
+        (r, c), (ld, one) = t.shape, t.stride()
+    except (AttributeError, ValueError):
+        _why(t, what, types, index, rows, cols)
+    if (on < 0 or t.dtype not in types or (one != 1 and c > 1) or (index is not None and on != index) or (rows is not None and r != rows)
+            or (cols is not None and c != cols) or (ld < c and r > 1) or (t.requires_grad and torch.is_grad_enabled())):
+        _why(t, what, types, index, rows, cols)
+    return r, c, ld if r > 1 else max(ld, c), on  # a single row's stride says nothing
 
 
-def _ld(t):
-    """Elements between the starts of two rows; a single row's stride says nothing."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _vector(t, what, types, index, n):
+    """The address of a contiguous vector of n values; None for None."""
+    if t is None:
+        return None
+    try:
+        if (t.get_device() != index or t.dtype not in types or t.shape != (n,) or (n > 1 and t.stride() != (1,))
+                or (t.requires_grad and torch.is_grad_enabled())):
+            _why(t, what, types, index, n)
+    except AttributeError:
+        _why(t, what, types, index, n)
+    return t.data_ptr()
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
+_stream = torch._C._cuda_getCurrentRawStream
+_F32, _I32, _I64, _I8 = (torch.float32,), (torch.int32,), (torch.int64,), (torch.int8,)
 
 
-def _stream(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def _codes(rows, dim, device):
+def _codes(x, rows, dim):
     """rows x dim int8 in rows of a multiple of 16 bytes, the padding zero: as linear reads them best."""
     wide = (dim + 15) // 16 * 16
     if wide == dim:
-        return torch.empty((rows, dim), dtype=torch.int8, device=device)
-    return torch.zeros((rows, wide), dtype=torch.int8, device=device)[:, :dim]
+        return x.new_empty((rows, dim), dtype=torch.int8)
+    return x.new_zeros((rows, wide), dtype=torch.int8)[:, :dim]
 
 
 def rms_norm_i8(x, gain=None, *, residual=None, eps: float = 1e-6, out_codes=None, out_scales=None, out_sum=None):
@@ -84,24 +96,26 @@ def rms_norm_i8(x, gain=None, *, residual=None, eps: float = 1e-6, out_codes=Non
     rounded to 8 bits; ``sum`` is ``h`` in the type of ``x`` (None without a residual).  ``gain`` is a
     vector of any of the three floating types.  ``out_sum`` may be ``x`` or ``residual`` itself.
     """
-    _ready(x, "x", _FLOATS)
-    rows, dim = x.shape
-    dev, t = x.device, (x.dtype,)
-    if gain is not None:
-        _shaped(gain, "gain", _FLOATS, dev, dim)
+    rows, dim, ldx, dev = _matrix(x, "x", _FLOATS)
+    kind = x.dtype
+    g = _vector(gain, "gain", _FLOATS, dev, dim)
+    r = ldr = 0
     if residual is not None:
-        _shaped(residual, "residual", t, dev, rows, dim)
+        ldr = _matrix(residual, "residual", (kind,), dev, rows, dim)[2]
+        r = residual.data_ptr()
+        if out_sum is None:
+            out_sum = x.new_empty((rows, dim))
+    s = lds = 0
     if out_sum is not None:
-        _shaped(out_sum, "out_sum", t, dev, rows, dim)
-    elif residual is not None:
-        out_sum = torch.empty((rows, dim), dtype=x.dtype, device=dev)
-    out_codes = _codes(rows, dim, dev) if out_codes is None else _shaped(out_codes, "out_codes", (torch.int8,), dev, rows, dim)
-    out_scales = torch.empty(rows, dtype=torch.float32, device=dev) if out_scales is None else _shaped(out_scales, "out_scales", (torch.float32,), dev, rows)
-    st = lib.lk_rms_norm_i8(dev.index, _FLOATS[x.dtype], rows, dim, x.data_ptr(), _ld(x),
-                            _p(residual), 0 if residual is None else _ld(residual),
-                            _p(gain), 0 if gain is None else _FLOATS[gain.dtype], eps,
-                            _p(out_sum), 0 if out_sum is None else _ld(out_sum),
-                            out_codes.data_ptr(), _ld(out_codes), out_scales.data_ptr(), _stream(dev))
+        lds = _matrix(out_sum, "out_sum", (kind,), dev, rows, dim)[2]
+        s = out_sum.data_ptr()
+    if out_codes is None:
+        out_codes = _codes(x, rows, dim)
+    if out_scales is None:
+        out_scales = x.new_empty(rows, dtype=torch.float32)
+    ldc = _matrix(out_codes, "out_codes", _I8, dev, rows, dim)[2]
+    st = lib.lk_rms_norm_i8(dev, _FLOATS[kind], rows, dim, x.data_ptr(), ldx, r, ldr, g, 0 if g is None else _FLOATS[gain.dtype], eps,
+                            s, lds, out_codes.data_ptr(), ldc, _vector(out_scales, "out_scales", _F32, dev, rows), _stream(dev))
     if st:
         check(st)
     return out_codes, out_scales, out_sum
@@ -115,19 +129,10 @@ def linear(a, w, *, a_scales=None, w_scales=None, bias=None, act: str = "none", 
     result: that of ``out``, else ``out_dtype``, else that of ``residual`` or ``bias``, else ``a``'s
     (float32 for int8).  ``out`` may be ``residual`` itself.  Rows on 16-byte boundaries run fastest.
     """
-    _ready(a, "a", _OPERANDS)
-    m, k = a.shape
-    dev = a.device
-    _ready(w, "w", (a.dtype,), dev)
-    n = w.shape[0]
-    if w.shape[1] != k:
-        _refuse(LK_EDIM, f"w: rows of {w.shape[1]} elements, those of a have {k}")
+    m, k, lda, dev = _matrix(a, "a", _OPERANDS)
+    n, _, ldw, _ = _matrix(w, "w", (a.dtype,), dev, None, k)
     if act not in ACTIVATIONS:
         _refuse(LK_EINVAL, f"act: one of {', '.join(ACTIVATIONS)}, not {act!r}")
-    if a_scales is not None:
-        _shaped(a_scales, "a_scales", (torch.float32,), dev, m)
-    if w_scales is not None:
-        _shaped(w_scales, "w_scales", (torch.float32,), dev, n)
     if out is not None:
         kind = out.dtype
         if out_dtype is not None and out_dtype != kind:
@@ -142,14 +147,17 @@ def linear(a, w, *, a_scales=None, w_scales=None, bias=None, act: str = "none", 
         kind = torch.float32 if a.dtype == torch.int8 else a.dtype
     if kind not in _FLOATS:
         _refuse(LK_EINVAL, f"out_dtype: {kind} is not supported here")
-    if bias is not None:
-        _shaped(bias, "bias", (kind,), dev, n)
+    r = ldr = 0
     if residual is not None:
-        _shaped(residual, "residual", (kind,), dev, m, n)
-    out = torch.empty((m, n), dtype=kind, device=dev) if out is None else _shaped(out, "out", (kind,), dev, m, n)
-    st = lib.lk_linear(dev.index, _OPERANDS[a.dtype], m, n, k, a.data_ptr(), _ld(a), _p(a_scales), w.data_ptr(), _ld(w), _p(w_scales),
-                       _p(bias), ACTIVATIONS[act], _p(residual), 0 if residual is None else _ld(residual),
-                       _FLOATS[kind], out.data_ptr(), _ld(out), _stream(dev))
+        ldr = _matrix(residual, "residual", (kind,), dev, m, n)[2]
+        r = residual.data_ptr()
+    sa, sw, b = _vector(a_scales, "a_scales", _F32, dev, m), _vector(w_scales, "w_scales", _F32, dev, n), _vector(bias, "bias", (kind,), dev, n)
+    if out is None:
+        out, ldo = a.new_empty((m, n), dtype=kind), n
+    else:
+        ldo = _matrix(out, "out", (kind,), dev, m, n)[2]
+    st = lib.lk_linear(dev, _OPERANDS[a.dtype], m, n, k, a.data_ptr(), lda, sa, w.data_ptr(), ldw, sw, b, ACTIVATIONS[act], r, ldr,
+                       _FLOATS[kind], out.data_ptr(), ldo, _stream(dev))
     if st:
         check(st)
     return out
@@ -161,11 +169,11 @@ def check_device(device=0):
     check(lib.lk_ops_status(index))
 
 
-def _per_row(v, what, dtype, rows, device):
-    """One value per row: a vector, or a number for all rows."""
-    if v is None or isinstance(v, torch.Tensor):
-        return v if v is None else _shaped(v, what, (dtype,), device, rows)
-    return torch.full((rows,), v, dtype=dtype, device=device)
+def _per_row(v, what, types, scores, rows, dev):
+    """(address, tensor) of one value per row: a vector, or a number for all rows."""
+    if v is not None and not isinstance(v, torch.Tensor):
+        v = scores.new_full((rows,), v, dtype=types[0])
+    return _vector(v, what, types, dev, rows), v
 
 
 def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, out_ids=None):
@@ -176,19 +184,18 @@ def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, o
     numbers for all rows; None switches a filter off.  ``probs`` is the probability of the draw among the
     ``kept`` entries.  A row with nothing to draw (only NaN and -inf) gets id -1.
     """
-    _ready(scores, "scores", _FLOATS)
-    rows, vocab = scores.shape
-    dev, f = scores.device, torch.float32
-    _shaped(u, "u", (f,), dev, rows)
-    temperature = _per_row(temperature, "temperature", f, rows, dev)
-    top_k = _per_row(top_k, "top_k", torch.int32, rows, dev)
-    top_p = _per_row(top_p, "top_p", f, rows, dev)
-    min_p = _per_row(min_p, "min_p", f, rows, dev)
-    ids = torch.empty(rows, dtype=torch.int64, device=dev) if out_ids is None else _shaped(out_ids, "out_ids", (torch.int64,), dev, rows)
-    probs = torch.empty(rows, dtype=f, device=dev)
-    kept = torch.empty(rows, dtype=torch.int32, device=dev)
-    st = lib.lk_sample(dev.index, _FLOATS[scores.dtype], rows, vocab, scores.data_ptr(), _ld(scores), _p(temperature), _p(top_k),
-                       _p(top_p), _p(min_p), u.data_ptr(), ids.data_ptr(), probs.data_ptr(), kept.data_ptr(), _stream(dev))
+    rows, vocab, ld, dev = _matrix(scores, "scores", _FLOATS)
+    up = _vector(u, "u", _F32, dev, rows)
+    t, hold_t = _per_row(temperature, "temperature", _F32, scores, rows, dev)
+    k, hold_k = _per_row(top_k, "top_k", _I32, scores, rows, dev)
+    p, hold_p = _per_row(top_p, "top_p", _F32, scores, rows, dev)
+    mp, hold_mp = _per_row(min_p, "min_p", _F32, scores, rows, dev)
+    if up is None:
+        _refuse(LK_EINVAL, "u: a CUDA tensor is wanted")
+    ids = scores.new_empty(rows, dtype=torch.int64) if out_ids is None else out_ids
+    probs, kept = scores.new_empty(rows, dtype=torch.float32), scores.new_empty(rows, dtype=torch.int32)
+    st = lib.lk_sample(dev, _FLOATS[scores.dtype], rows, vocab, scores.data_ptr(), ld, t, k, p, mp, up,
+                       _vector(ids, "out_ids", _I64, dev, rows), probs.data_ptr(), kept.data_ptr(), _stream(dev))
     if st:
         check(st)
     return ids, probs, kept
