@@ -1,22 +1,26 @@
 // One draw per row of scores: temperature, top-k, top-p, min-p, from given random numbers.
 //
 // Every filter keeps a prefix of the row's order (score descending, index ascending), so what is kept is
-// described by its last entry: a 64-bit ranking key (score image, ~index) at or above which entries are kept.  No
-// sort is needed; a cut is found by histograms over the order, with counts (top-k) or weights (top-p).
-//
-// Weights w = exp((x - max) / T) are computed in float64 and summed as 64-bit integers, w * 2^F with
-// vocab * 2^F <= 2^63: sums do not depend on their order (shared-memory atomics, warps, CTAs), the prefix that a
-// cut finds and the running sum that a draw walks agree to the last bit, and a border between two entries
-// is met to ~2^-44 of the largest weight.
+// described by its last entry: a 64-bit ranking key (score image, ~index) at or above which entries are kept.
+// Weights w = exp((x - max) / T) are computed in float64 and summed as 64-bit integers, w * 2^F with vocab *
+// 2^F <= 2^63 and F <= 50: sums do not depend on their order (shared-memory atomics, warps, CTAs), the prefix
+// that a cut finds and the running sum that a draw walks agree to the last bit, and a border between two
+// entries is met to ~2^-F of the largest weight.
 //
 // A cluster of CTAs owns a row.  Each loads one stretch of it into its shared memory (what does not fit is read
 // again from L2), so scores cross HBM once; every later pass runs over shared memory, and the CTAs
-// exchange maxima, histograms and sums through distributed shared memory.
+// exchange maxima, histograms and sums through distributed shared memory.  Bound: instructions per entry
+// and pass, so passes are what is saved:
 //
-// A cut: entries fall into 1,024 bins by the distance d = max - x, 32 bins to a factor of two (the image
-// of d without its low bits: monotone in x, and fine where a softmax has its weight).  The bin in which the
-// measure reaches its target is cut again: up to 1,024 entries are gathered in one CTA, where each counts
-// what ranks above it; more are binned again by their images; entries that are all equal are cut by index.
+// * Few candidates.  With a top-k, the k-th largest of the threads' maxima bounds the k-th score from below: one
+//   pass gathers what reaches that bound in one CTA, and if that is 1,024 entries or fewer they are sorted there and
+//   all filters and the draw are settled among them.  Without a top-k the same happens when the bins that
+//   hold top_p of the weight have that few entries.
+// * Many.  A cut by count or weight: entries fall into 1,024 bins by the distance d = max - x, 32 bins to a
+//   factor of two (the bits of d without the low ones: monotone in x, and fine where a softmax has its
+//   weight).  The bin in which the measure reaches its target is cut again by the next bits of d, then by the
+//   bits of x, until at most 1,024 entries are left to be sorted, or all are equal and are cut by index.
+//   Then a pass sums the kept weights by warp and CTA, and the draw walks down those sums.
 #include "devops.cuh"
 
 namespace lk {
@@ -31,27 +35,30 @@ struct SampleArgs {
     long long *ids;
     float *probs;
     int *kept;
-    double unit;  // 2^F
+    int unit_bits;  // F
 };
 
 constexpr unsigned kNegInf = 0x007fffffu;  // image of -infinity; NaN (0) is below it
 constexpr int ST = 1024, SWARPS = ST / 32;
-constexpr int SBINS = 1024;
-constexpr int SLIST = 1024;
+constexpr int SBINS = 1024;                // one thread per bin
+constexpr int SLIST = 1024;                // one thread per candidate
 constexpr int SMAX_CTAS = 16;
+constexpr int SD_SHIFT = 18, SD_BASE = (127 - 16) << 5;  // bins by d: exponent and 5 bits, from 2^-16 to 2^16
 using u64 = unsigned long long;
 
 struct alignas(16) SampleShared {
     unsigned lo[SBINS], hi[SBINS], n[SBINS];   // this CTA's bins: weights (two words), entries
     u64 all_w[SBINS];                          // the row's bins
     unsigned all_n[SBINS];
-    u64 list[SLIST];                           // the leader's: keys of the bin being cut
+    u64 list[SLIST];                           // the first CTA's: candidates
+    u64 sorted[SLIST];
+    double octave[32];                         // 2^(j/32)
     u64 warp_w[SWARPS];
     unsigned warp_n[SWARPS];
     u64 slot_w[SMAX_CTAS];                     // one word from every CTA of the row
     unsigned slot_a[SMAX_CTAS], slot_b[SMAX_CTAS];
     unsigned listed;
-    u64 cut;                                   // a decision of the leader or of the CTA that holds an entry
+    u64 cut;                                   // a decision of the first CTA, or of the one that holds an entry
     u64 found_w, found_before;
     int found;
 };
@@ -90,14 +97,19 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {  // inclusive
 // One row, as the CTAs of its cluster see it.
 template <typename T>
 struct Row {
+    static constexpr int PER = 16 / sizeof(T);  // entries of a 16-byte group
     const SampleArgs &a;
     SampleShared &s;
-    T *data;        // this CTA's stretch in shared memory, `cap` entries of it
-    const T *x;     // the row
+    T *data;        // this CTA's stretch in shared memory, `cap` entries of it, padded with NaN to a whole group
+    const T *x;     // this CTA's stretch in global memory
     int rank, start, len, wlen, tid, lane, warp;
-    unsigned top;
-    double x_top, per_t;
+    float top;      // the largest score
+    double octaves; // 32 / (T ln 2): a distance in 32nds of an octave
+    float least;    // min_p, and its logarithm
+    double log_least;
     u64 thr;        // entries with a key at or above this are kept
+    float thr_x;    // its score and its index
+    unsigned thr_i;
 
     __device__ __forceinline__ void sync() const {
         if (a.ctas > 1) {
@@ -106,28 +118,62 @@ struct Row {
         } else
             __syncthreads();
     }
-    __device__ __forceinline__ unsigned image(int i) const { return ord_from_f32(Elem<T>::get(i < a.cap ? data[i] : x[start + i])); }
-    __device__ __forceinline__ double weight(unsigned o) const {
-        return o == top ? 1.0 : exp(((double)f32_from_ord(o) - x_top) * per_t);
+    __device__ __forceinline__ u64 key(float v, int i) const { return make_key(ord_from_f32(v), (unsigned)(start + i)); }
+    __device__ __forceinline__ void keep_from(u64 k) {
+        thr = k;
+        thr_x = f32_from_ord(key_ord(k));
+        thr_i = key_slot(k);
     }
-    __device__ __forceinline__ u64 whole(double w) const { return __double2ull_rn(w * a.unit); }
-    __device__ __forceinline__ u64 key(unsigned o, int i) const { return make_key(o, (unsigned)(start + i)); }
+    // NaN compares false; -infinity is below every threshold
+    __device__ __forceinline__ bool kept(float v, int i) const { return v > thr_x || (v == thr_x && (unsigned)(start + i) <= thr_i); }
+    __device__ __forceinline__ float entry(int i) const { return Elem<T>::get(i < a.cap ? data[i] : x[i]); }
 
-    // f(image, local index) for every entry of this warp; lanes past the end see image 0 (never kept)
+    // w * 2^F of a score, rounded.  Tang's scheme (ACM TOMS 15, 1989): with y = (x - max) / T / ln 2 * 32 = n + r, n whole,
+    // |r| <= 1/2:  w = 2^(n div 32) * 2^((n mod 32) / 32) * e^(r ln 2 / 32), the middle factor from a table, the last by its
+    // series to the fifth power (next term 2e-15).  The widening of x and both roundings to whole numbers are done by
+    // adding constants and on the bits: conversions issue at an eighth of the rate.
+    __device__ __forceinline__ u64 weight(float v) const {
+        if (v == top) return 1ull << a.unit_bits;
+        if (!((v - top) * (float)octaves >= -32.0f * 64.0f)) return 0ull;  // below 2^-64 of the largest; an infinite distance too
+        const auto wide = [](float f) -> double {
+            const unsigned b = __float_as_uint(f);
+            if ((b & 0x7f800000u) == 0u) return (double)f;  // zero and subnormals
+            return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + (896u << 20))), (int)(b << 29));
+        };
+        const double whole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number in the low word
+        const double dx = wide(v) - wide(top);
+        const double t = fma(dx, octaves, whole);
+        const double r = fma(dx, octaves, -(t - whole));
+        const int n = __double2loint(t);
+        constexpr double c = 0.693147180559945309417232 / 32;
+        double q = fma(r, c * c * c * c * c / 120, c * c * c * c / 24);
+        q = fma(r, q, c * c * c / 6);
+        q = fma(r, q, c * c / 2);
+        q = fma(r, q, c);
+        q = fma(r, q, 1.0);
+        const double scale = __hiloint2double((1023 + (n >> 5) + a.unit_bits) << 20, 0);
+        const double w = fma(s.octave[n & 31] * q, scale, 4503599627370496.0);  // + 2^52; w <= 2^50
+        return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+    }
+
+    // f(score, local index) for every entry of this warp's stretch; a stretch is whole groups but for the row's end
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
-        const int lo = warp * wlen, hi = min(lo + wlen, len);
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            const int i = i0 + lane;
-            f(i < hi ? image(i) : 0u, i);
+        const int lo = warp * wlen, hi = min(lo + wlen, len), held = min(hi, a.cap);
+        for (int i = lo + lane * PER; i < held; i += 32 * PER) {
+            const uint4 q = *reinterpret_cast<const uint4 *>(data + i);
+            const T *t = reinterpret_cast<const T *>(&q);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) f(Elem<T>::get(t[e]), i + e);
         }
+        for (int i = max(lo, a.cap) + lane; i < hi; i += 32) f(Elem<T>::get(x[i]), i);
     }
 
     // Sum of f over the row, by integers; warp_w keeps this CTA's warps' sums and slot_w the CTAs'.
     template <typename F>
-    __device__ u64 sums(F f) const {
+    __device__ __forceinline__ u64 sums(F f) const {
         u64 w = 0;
-        each([&](unsigned o, int i) { w += f(o, i); });
+        each([&](float v, int i) { w += f(v, i); });
         w = warp_sum(w);
         __syncthreads();
         if (lane == 0) s.warp_w[warp] = w;
@@ -142,10 +188,10 @@ struct Row {
         return all;
     }
     // The entry at which the running sum of f (in the order of the indexes) first exceeds `target`, which
-    // is below the sum that sums(f) has just returned: the CTA that holds it sets found (local index),
-    // found_w (its f) and found_before; in the others found is -1.  No meeting of the cluster.
+    // is below the sum that sums(f) has just returned: the CTA that holds it sets found (local index) and
+    // found_w (its f); in the others found is -1.  No meeting of the cluster.
     template <typename F>
-    __device__ void walk(F f, u64 target) const {
+    __device__ __forceinline__ void walk(F f, u64 target) const {
         __syncthreads();
         if (tid == 0) s.found = -1;
         u64 before = 0;
@@ -166,7 +212,7 @@ struct Row {
             u64 w = 0;
             for (int i0 = lo + warp * n; i0 < min(lo + (warp + 1) * n, end); i0 += 32) {
                 const int i = i0 + lane;
-                if (i < end) w += f(image(i), i);
+                if (i < end) w += f(entry(i), i);
             }
             w = warp_sum(w);
             __syncthreads();
@@ -176,11 +222,11 @@ struct Row {
         if (warp == 0) {
             for (int i0 = lo; i0 < min(lo + n, len); i0 += 32) {
                 const int i = i0 + lane;
-                const u64 w = i < len ? f(image(i), i) : 0ull;
+                const u64 w = i < len ? f(entry(i), i) : 0ull;
                 const u64 inc = warp_scan(w, lane) + before;
                 const unsigned past = __ballot_sync(0xffffffffu, inc > target);
                 if (past) {
-                    if (lane == __ffs(past) - 1) s.found = i, s.found_w = w, s.found_before = inc - w;
+                    if (lane == __ffs(past) - 1) s.found = i, s.found_w = w;
                     break;
                 }
                 before = __shfl_sync(0xffffffffu, inc, 31);
@@ -189,100 +235,211 @@ struct Row {
         __syncthreads();
     }
 
-    // The bin of an entry: by distance, or by image within [olo, ohi] (equal steps of 2^shift).
-    __device__ __forceinline__ int bin(unsigned o, unsigned ohi, int shift) const {
-        if (shift >= 0) return (int)((ohi - o) >> shift);
-        const float d = o == top ? 0.0f : f32_from_ord(top) - f32_from_ord(o);
-        return min(max((int)(__float_as_uint(d) >> 18) - ((127 - 16) << 5), 0), SBINS - 1);
+    // Keys sorted, largest first, one per thread (0 = none); every thread of the CTA takes part.  Strides below 32 by
+    // shuffles, wider ones through shared memory.
+    __device__ __forceinline__ u64 sort(u64 k, int n) const {
+        int size_max = 32;
+        while (size_max < n) size_max <<= 1;
+        for (int size = 2; size <= size_max; size <<= 1) {
+            const bool down = (tid & size) == 0;  // this stretch descends
+            for (int stride = size >> 1; stride > 0; stride >>= 1) {
+                u64 o;
+                if (stride >= 32) {
+                    __syncthreads();
+                    s.sorted[tid] = k;
+                    __syncthreads();
+                    o = s.sorted[tid ^ stride];
+                } else
+                    o = shfl_xor_u64(k, stride);
+                const bool low = (tid & stride) == 0;
+                if ((k < o) == (low == down)) k = o;
+            }
+        }
+        return k;
+    }
+    // Inclusive running sum over the threads of the CTA.
+    __device__ __forceinline__ u64 block_scan(u64 v) const {
+        v = warp_scan(v, lane);
+        __syncthreads();
+        if (lane == 31) s.warp_w[warp] = v;
+        __syncthreads();
+        const u64 other = warp_scan(s.warp_w[lane], lane);
+        return warp == 0 ? v : v + __shfl_sync(0xffffffffu, other, warp - 1);
     }
 
-    // Moves thr up to the last entry of the shortest prefix whose measure reaches `want` (>= 1): MASS: the
-    // weight, else the number of entries.  A prefix that never reaches it is left as it is.
+    // The first CTA has every entry that may be kept in its list (n of them): all filters, and the draw.  `all`: the weight
+    // that top_p refers to, 0 = that of the k first.
+    __device__ void finish(long long row, int n, int k, float p, float u, u64 all) const {
+        const u64 mine = sort(tid < n ? s.list[tid] : 0ull, n);  // thread t holds the entry of rank t
+        const float v = f32_from_ord(key_ord(mine));
+        const bool in = tid < n && (k <= 0 || tid < k);
+        const u64 w = in ? weight(v) : 0ull;
+        const u64 inc = block_scan(w);
+        if (tid == ST - 1) s.found_before = inc;
+        __syncthreads();
+        if (all == 0) all = s.found_before;
+        const u64 want = p < 1.0f ? (p <= 0.0f ? 1ull : max((u64)ceil((double)p * (double)all), (u64)1)) : ~0ull;
+        const bool keep = in && inc - w < want && (tid == 0 || likely(v));
+        const int count = __syncthreads_count(keep);
+        if (tid == count - 1) s.found_w = inc;
+        s.all_w[tid] = w;
+        const unsigned slot = key_slot(mine);
+        // the kept ones by index: largest first of ~(index, rank)
+        const u64 by_index = sort(keep ? ~(((u64)slot << 10) | (unsigned)tid) : 0ull, count);
+        __syncthreads();
+        const u64 total = s.found_w;
+        const unsigned from = (unsigned)~by_index & 1023u;
+        const u64 w2 = tid < count ? s.all_w[from] : 0ull;
+        const u64 run = block_scan(w2);
+        const u64 target = aim(u, total);
+        if (run - w2 <= target && target < run) {
+            a.ids[row] = (long long)((~by_index) >> 10);
+            if (a.probs) a.probs[row] = (float)((double)w2 / (double)total);
+            if (a.kept) a.kept[row] = count;
+        }
+    }
+    // w >= min_p, as (x - max) / T >= log(min_p)
+    __device__ __forceinline__ bool likely(float v) const {
+        return least <= 0.0f || v == top || ((double)v - (double)top) * (octaves * (0.693147180559945309417232 / 32)) >= log_least;
+    }
+    static __device__ __forceinline__ u64 aim(float u, u64 total) {
+        const double t = (double)u * (double)total;
+        return t <= 0.0 ? 0ull : (t >= (double)total ? total - 1 : min((u64)t, total - 1));
+    }
+
+    // Every CTA adds up its share of the row's bins and hands the sums to all.
     template <bool MASS>
-    __device__ void cut(u64 want) {
-        unsigned olo = 0, ohi = ~0u;
-        int shift = -1;
-        u64 base = 0;  // measure of what lies above [olo, ohi]
-        for (;;) {
-            for (int b = tid; b < SBINS; b += ST) {
-                s.n[b] = 0;
-                if (MASS) s.lo[b] = s.hi[b] = 0;
+    __device__ __forceinline__ void join_bins() const {
+        sync();
+        const int share = (SBINS + a.ctas - 1) / a.ctas;
+        for (int b = rank * share + tid; b < min((rank + 1) * share, SBINS); b += ST) {
+            unsigned n = 0;
+            u64 w = 0;
+            for (int r = 0; r < a.ctas; ++r) {
+                n += s_get(s_at(&s.n[b], r));
+                if (MASS) w += ((u64)s_get(s_at(&s.hi[b], r)) << 32) + s_get(s_at(&s.lo[b], r));
             }
-            if (tid == 0) s.listed = 0;
-            __syncthreads();
-            each([&](unsigned o, int i) {
-                if (o < olo || o > ohi || key(o, i) < thr) return;
-                const int b = bin(o, ohi, shift);
+            for (int r = 0; r < a.ctas; ++r) {
+                s_put(s_at(&s.all_n[b], r), n);
+                if (MASS) s_put(s_at(&s.all_w[b], r), w);
+            }
+        }
+        sync();
+    }
+    template <bool MASS>
+    __device__ __forceinline__ void clear_bins() const {
+        s.n[tid] = 0;
+        if (MASS) s.lo[tid] = s.hi[tid] = 0;
+        if (tid == 0) s.listed = 0;
+        __syncthreads();
+    }
+    // The bin in which the running measure (from `base` on) reaches `want`, -1 if none; found_before = what lies above it.
+    __device__ __forceinline__ int reach(u64 m, u64 base, u64 want) const {
+        if (tid == 0) s.found = -1;
+        const u64 inc = block_scan(m) + base;
+        if (inc >= want && inc - m < want) s.found = tid, s.found_before = inc - m;
+        __syncthreads();
+        return s.found;
+    }
+    __device__ __forceinline__ unsigned distance(float v) const { return __float_as_uint(v == top ? 0.0f : top - v); }
+    static __device__ __forceinline__ int first_bin(unsigned d) { return min(max((int)(d >> SD_SHIFT) - SD_BASE, 0), SBINS - 1); }
+
+    // The candidates of bin b and above, in the first CTA's list: d below an end.  Their number (which may be more than fit).
+    __device__ __forceinline__ unsigned gather_to(int b) const {
+        const unsigned end = (unsigned)(SD_BASE + b + 1) << SD_SHIFT;
+        const float before = b >= SBINS - 1 ? CUDART_INF_F : __uint_as_float(end);
+        each([&](float v, int i) {
+            if (top - v < before || v == top) {  // false for NaN and -infinity
+                const unsigned at = s_add(s_at(&s.listed, 0), 1u);
+                if (at < SLIST) s_put(s_at(&s.list[at], 0), key(v, i));
+            }
+        });
+        sync();
+        return s_get(s_at(&s.listed, 0));
+    }
+
+    // MASS: moves thr up to the last entry of the shortest prefix that holds the share p of the kept weight.
+    // Else: to the k-th entry.  Returns the number of candidates when all that may be kept is in the first
+    // CTA's list instead (`whole`: thr is still at the row's end), with the row's weight in *all; 0 when thr has been moved.
+    template <bool MASS>
+    __device__ int cut(int k, float p, bool whole, u64 *all) {
+        u64 want = (u64)k, base = 0;  // base: measure of what lies above the current bin
+        // the entries looked at: d >> in == pre (by distance), or image in [olo, ohi]; their bins: (d >> sub) - from
+        int in = 31, sub = SD_SHIFT;
+        unsigned pre = 0, from = SD_BASE, olo = 0, ohi = 0;
+        bool by_image = false;
+        for (int level = 0;; ++level) {
+            clear_bins<MASS>();
+            const auto bin = [&](float v) -> int {  // -1: not among those looked at
+                if (by_image) {
+                    const unsigned o = ohi - ord_from_f32(v);
+                    return o <= ohi - olo ? (int)(o >> sub) : -1;
+                }
+                const unsigned d = distance(v);
+                return (d >> in) == pre ? min(max((int)(d >> sub) - (int)from, 0), SBINS - 1) : -1;
+            };
+            each([&](float v, int i) {
+                if (!kept(v, i)) return;
+                const int b = bin(v);
+                if (b < 0) return;
                 atomicAdd(&s.n[b], 1u);
                 if (MASS) {
-                    const u64 w = whole(weight(o));
+                    const u64 w = weight(v);
                     const unsigned l = (unsigned)w, old = atomicAdd(&s.lo[b], l);
                     const unsigned h = (unsigned)(w >> 32) + (old + l < l ? 1u : 0u);
                     if (h) atomicAdd(&s.hi[b], h);
                 }
             });
-            sync();
-            // every CTA adds up its share of the bins and hands the sums to all
-            const int share = (SBINS + a.ctas - 1) / a.ctas;
-            for (int b = rank * share + tid; b < min((rank + 1) * share, SBINS); b += ST) {
-                unsigned n = 0;
-                u64 w = 0;
-                for (int r = 0; r < a.ctas; ++r) {
-                    n += s_get(s_at(&s.n[b], r));
-                    if (MASS) w += ((u64)s_get(s_at(&s.hi[b], r)) << 32) + s_get(s_at(&s.lo[b], r));
-                }
-                for (int r = 0; r < a.ctas; ++r) {
-                    s_put(s_at(&s.all_n[b], r), n);
-                    if (MASS) s_put(s_at(&s.all_w[b], r), w);
-                }
-            }
-            sync();
-            // the bin that reaches the target: thread t holds bin t
+            join_bins<MASS>();
             const u64 m = MASS ? s.all_w[tid] : (u64)s.all_n[tid];
-            u64 inc = warp_scan(m, lane);
-            if (tid == 0) s.found = -1;
-            if (lane == 31) s.warp_w[warp] = inc;
-            __syncthreads();
-            u64 run = base;
-            for (int w = 0; w < warp; ++w) run += s.warp_w[w];
-            inc += run;
-            if (inc >= want && inc - m < want) s.found = tid, s.found_before = inc - m;
-            __syncthreads();
-            const int b = s.found;
-            if (b < 0) return;  // all of it does not reach the target
+            if (MASS && level == 0) {
+                const u64 inc = block_scan(m);
+                if (tid == ST - 1) s.cut = inc;
+                __syncthreads();
+                *all = s.cut;
+                want = p <= 0.0f ? 1ull : max((u64)ceil((double)p * (double)*all), (u64)1);
+            }
+            const int b = reach(m, base, want);
+            if (b < 0) return 0;  // fewer entries than k: all are kept
             base = s.found_before;
             const unsigned n = s.all_n[b];
+            if (level == 0 && whole) {  // everything down to this bin
+                const u64 upto = block_scan(tid <= b ? s.all_n[tid] : 0u);
+                if (tid == ST - 1) s.found_w = upto;
+                __syncthreads();
+                if (s.found_w <= SLIST && b < SBINS - 1) return (int)gather_to(b);
+            }
             if (n <= SLIST) {
-                each([&](unsigned o, int i) {
-                    const bool in = o >= olo && o <= ohi && key(o, i) >= thr && bin(o, ohi, shift) == b;
-                    const unsigned who = __ballot_sync(0xffffffffu, in);
-                    if (who == 0) return;
-                    unsigned at = 0;
-                    if (lane == __ffs(who) - 1) at = s_add(s_at(&s.listed, 0), __popc(who));
-                    at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1) + __popc(who & lanemask_lt());
-                    if (in) s_put(s_at(&s.list[at], 0), key(o, i));
+                each([&](float v, int i) {
+                    if (kept(v, i) && bin(v) == b) s_put(s_at(&s.list[s_add(s_at(&s.listed, 0), 1u)], 0), key(v, i));
                 });
                 sync();
-                if (rank == 0) {  // what ranks above mine?  one entry is the last that is needed
-                    const u64 k = tid < (int)n ? s.list[tid] : 0ull;
-                    if (MASS) {  // the weights beside the keys
-                        if (tid < (int)n) s.all_w[tid] = whole(weight(key_ord(k)));
-                        __syncthreads();
-                    }
-                    u64 above = base;
-                    for (unsigned e = 0; e < n; ++e)
-                        if (s.list[e] > k) above += MASS ? s.all_w[e] : 1ull;
-                    if (tid < (int)n && above < want && above + (MASS ? s.all_w[tid] : 1ull) >= want)
-                        for (int r = 0; r < a.ctas; ++r) s_put(s_at(&s.cut, r), k);
+                if (rank == 0) {
+                    const u64 mine = sort(tid < (int)n ? s.list[tid] : 0ull, (int)n);
+                    const u64 w = tid >= (int)n ? 0ull : (MASS ? weight(f32_from_ord(key_ord(mine))) : 1ull);
+                    const u64 inc = block_scan(w) + base;
+                    if (inc >= want && inc - w < want)
+                        for (int r = 0; r < a.ctas; ++r) s_put(s_at(&s.cut, r), mine);
                 }
                 sync();
-                thr = s.cut;
-                return;
+                keep_from(s.cut);
+                return 0;
             }
-            // too many: how far apart are they?
+            // too many: the next bits of the distance, where the bin is one value of the bits above
+            if (!by_image && sub > 0 && (level > 0 || (b > 0 && b < SBINS - 1))) {
+                in = sub;
+                pre = from + (unsigned)b;
+                sub = sub == SD_SHIFT ? 8 : 0;
+                from = pre << (in - sub);
+                continue;
+            }
+            // the bits of the scores, between the least and the largest of the bin
             unsigned least = ~0u, most = 0;
-            each([&](unsigned o, int i) {
-                if (o >= olo && o <= ohi && key(o, i) >= thr && bin(o, ohi, shift) == b) least = min(least, o), most = max(most, o);
+            each([&](float v, int i) {
+                if (kept(v, i) && bin(v) == b) {
+                    const unsigned o = ord_from_f32(v);
+                    least = min(least, o), most = max(most, o);
+                }
             });
             least = __reduce_min_sync(0xffffffffu, least);
             most = __reduce_max_sync(0xffffffffu, most);
@@ -302,22 +459,24 @@ struct Row {
             for (int r = 0; r < a.ctas; ++r) olo = min(olo, s.slot_a[r]), ohi = max(ohi, s.slot_b[r]);
             sync();  // the slots may be written again
             if (olo == ohi) {  // equal scores: the first of them, by index
-                const u64 each_w = MASS ? whole(weight(olo)) : 1ull;
+                const float tied = f32_from_ord(olo);
+                const u64 each_w = MASS ? weight(tied) : 1ull;
                 const u64 need = (want - base + each_w - 1) / each_w;  // each_w > 0: the bin reaches the target
                 if (need < n) {
-                    const auto tie = [&](unsigned o, int i) -> u64 { return o == olo && key(o, i) >= thr; };
+                    const auto tie = [&](float v, int i) -> u64 { return v == tied && kept(v, i); };
                     sums(tie);
                     walk(tie, need - 1);
                     if (tid == 0 && s.found >= 0)
-                        for (int r = 0; r < a.ctas; ++r) s_put(s_at(&s.cut, r), key(olo, s.found));
+                        for (int r = 0; r < a.ctas; ++r) s_put(s_at(&s.cut, r), key(tied, s.found));
                     sync();
-                    thr = s.cut;
+                    keep_from(s.cut);
                 } else
-                    thr = max(thr, (u64)make_key(olo, ~0u));
-                return;
+                    keep_from(max(thr, (u64)make_key(olo, ~0u)));
+                return 0;
             }
-            shift = 0;
-            while (((ohi - olo) >> shift) >= SBINS) ++shift;
+            by_image = true;
+            sub = 0;
+            while (((ohi - olo) >> sub) >= SBINS) ++sub;
         }
     }
 };
@@ -328,29 +487,31 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     SampleShared &s = *reinterpret_cast<SampleShared *>(s_raw);
     const long long row = blockIdx.x / a.ctas;
     const int rank = blockIdx.x % a.ctas;  // the cluster is the row's CTAs, in order
-    Row<T> w = {a, s, reinterpret_cast<T *>(s_raw + sizeof(SampleShared)), static_cast<const T *>(a.logits) + row * a.ld};
+    const int start = min(rank * a.seg, a.vocab);
+    Row<T> w = {a, s, reinterpret_cast<T *>(s_raw + sizeof(SampleShared)), static_cast<const T *>(a.logits) + row * a.ld + start};
+    constexpr int PER = Row<T>::PER;
     const int tid = w.tid = threadIdx.x, lane = w.lane = tid & 31, warp = w.warp = tid >> 5;
     w.rank = rank;
-    w.start = min(rank * a.seg, a.vocab);
-    w.len = min(a.seg, a.vocab - w.start);
-    w.wlen = ((w.len + SWARPS - 1) / SWARPS + 31) & ~31;
+    w.start = start;
+    w.len = min(a.seg, a.vocab - start);
+    w.wlen = (int)round_up((w.len + SWARPS - 1) / SWARPS, PER);
 
     float temp = a.temperature ? a.temperature[row] : 1.0f;
     int k = a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f;
     const float least_in = a.min_p ? a.min_p[row] : 0.0f;
-    const float least = fminf(least_in, 1.0f);  // the first is always kept
+    w.least = fminf(least_in, 1.0f);  // the first is always kept
+    w.log_least = w.least > 0.0f ? log((double)w.least) : 0.0;
     const float u = a.u[row];
     const bool bad = !(temp >= 0.0f) || p != p || least_in != least_in || u != u;
     if (temp == 0.0f) temp = 1.0f, k = 1;
+    if (warp == 1) s.octave[lane] = exp2(lane / 32.0);
 
     // ---- the row comes in; its largest score ----
-    const T *x = w.x + w.start;
     const int held = min(w.len, a.cap);
-    unsigned top = 0;
-    constexpr int PER = 16 / sizeof(T);
+    unsigned own = 0;  // the largest that this thread has seen
     int done = 0;
-    if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+    if ((reinterpret_cast<uintptr_t>(w.x) & 15) == 0) {
         const int vecs = held / PER;
         done = vecs * PER;
         constexpr int U = 4;
@@ -358,23 +519,24 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
             uint4 q[U];
 #pragma unroll
             for (int e = 0; e < U; ++e)
-                if (v0 + e * ST < vecs) q[e] = reinterpret_cast<const uint4 *>(x)[v0 + e * ST];
+                if (v0 + e * ST < vecs) q[e] = reinterpret_cast<const uint4 *>(w.x)[v0 + e * ST];
 #pragma unroll
             for (int e = 0; e < U; ++e)
                 if (v0 + e * ST < vecs) {
                     reinterpret_cast<uint4 *>(w.data)[v0 + e * ST] = q[e];
                     const T *t = reinterpret_cast<const T *>(&q[e]);
 #pragma unroll
-                    for (int i = 0; i < PER; ++i) top = max(top, ord_from_f32(Elem<T>::get(t[i])));
+                    for (int i = 0; i < PER; ++i) own = max(own, ord_from_f32(Elem<T>::get(t[i])));
                 }
         }
     }
     for (int i = done + tid; i < w.len; i += ST) {
-        const T t = x[i];
+        const T t = w.x[i];
         if (i < held) w.data[i] = t;
-        top = max(top, ord_from_f32(Elem<T>::get(t)));
+        own = max(own, ord_from_f32(Elem<T>::get(t)));
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    for (int i = held + tid; i < (int)round_up(held, PER); i += ST) w.data[i] = Elem<T>::put(CUDART_NAN_F);
+    unsigned top = __reduce_max_sync(0xffffffffu, own);
     if (lane == 0) s.warp_n[warp] = top;
     if (a.ctas > 1) w.sync();  // every CTA of the cluster runs before any writes to another
     else __syncthreads();
@@ -390,53 +552,63 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
             if (a.probs) a.probs[row] = 0.0f;
             if (a.kept) a.kept[row] = 0;
         }
-        if (a.ctas > 1) w.sync();
-        return;
+        return;  // nothing is written to this CTA any more
     }
-    w.top = top;
-    w.x_top = (double)f32_from_ord(top);
-    w.per_t = fmax(1.0 / (double)temp, 1e-300);  // never 0: an infinite distance stays one
-    w.thr = make_key(kNegInf + 1, ~0u);
+    w.top = f32_from_ord(top);
+    w.octaves = fmin(fmax(32.0 / (0.693147180559945309417232 * (double)temp), 1e-300), 1e300);  // an infinite distance stays one
+    w.keep_from(make_key(kNegInf + 1, 0xffffffffu - 1u));
     w.sync();  // the slots may be written again
 
+    // ---- few candidates ----
+    int n = 0;
+    u64 all = 0;
+    if (k > 0 && k <= SLIST / 2) {
+        w.template clear_bins<false>();
+        if (own > kNegInf) atomicAdd(&s.n[Row<T>::first_bin(w.distance(f32_from_ord(own)))], 1u);
+        w.template join_bins<false>();
+        const int b = w.reach(s.all_n[tid], 0, (u64)k);
+        if (b >= 0 && b < SBINS - 1) n = (int)w.gather_to(b);
+        if (n > SLIST) n = 0;
+        w.sync();  // the count has been read
+    }
     // ---- the cuts ----
-    if (k > 0 && k < a.vocab) w.template cut<false>((u64)k);
-    if (p < 1.0f) {
-        const u64 all = w.sums([&](unsigned o, int i) -> u64 { return w.key(o, i) >= w.thr ? w.whole(w.weight(o)) : 0ull; });
-        w.sync();
-        w.template cut<true>(p <= 0.0f ? 1ull : max((u64)ceil((double)p * (double)all), (u64)1));
+    if (n == 0) {
+        const bool by_count = k > 0 && k < a.vocab;
+        if (by_count) w.template cut<false>(k, 1.0f, false, &all);
+        if (p < 1.0f) n = w.template cut<true>(0, p, !by_count, &all);
+    }
+    if (n > 0) {
+        if (rank == 0) w.finish(row, n, k, p, u, all);
+        if (a.ctas > 1) w.sync();  // the others' shared memory is not needed any more, but was read above
+        return;
     }
 
     // ---- the draw ----
-    u64 count = 0;
-    const auto kept_weight = [&](unsigned o, int i) -> u64 {
-        if (w.key(o, i) < w.thr) return 0ull;
-        const double v = w.weight(o);
-        if (least > 0.0f && v < (double)least) return 0ull;
+    unsigned count = 0;
+    const auto kept_weight = [&](float v, int i) -> u64 {
+        if (!w.kept(v, i) || !w.likely(v)) return 0ull;
         ++count;
-        return w.whole(v);
+        return w.weight(v);
     };
-    const u64 all = w.sums(kept_weight);
-    count = warp_sum(count);
-    if (lane == 0) s.warp_n[warp] = (unsigned)count;
-    const double t = (double)u * (double)all;
-    const u64 target = t <= 0.0 ? 0ull : (t >= (double)all ? all - 1 : min((u64)t, all - 1));
-    w.walk(kept_weight, target);
+    all = w.sums(kept_weight);
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (lane == 0) s.warp_n[warp] = count;
+    w.walk(kept_weight, Row<T>::aim(u, all));
     __syncthreads();
     if (s.found >= 0 && tid == 0) {
-        a.ids[row] = w.start + s.found;
+        a.ids[row] = start + s.found;
         if (a.probs) a.probs[row] = (float)((double)s.found_w / (double)all);
     }
     if (a.kept) {
         if (warp == 0) {
-            const unsigned n = __reduce_add_sync(0xffffffffu, s.warp_n[lane]);
-            if (lane == 0) s_put(s_at(&s.slot_b[rank], 0), n);
+            const unsigned c = __reduce_add_sync(0xffffffffu, s.warp_n[lane]);
+            if (lane == 0) s_put(s_at(&s.slot_b[rank], 0), c);
         }
         w.sync();
         if (rank == 0 && tid == 0) {
-            unsigned n = 0;
-            for (int r = 0; r < a.ctas; ++r) n += s.slot_b[r];
-            a.kept[row] = (int)n;
+            unsigned c = 0;
+            for (int r = 0; r < a.ctas; ++r) c += s.slot_b[r];
+            a.kept[row] = (int)c;
         }
     }
 }
@@ -509,7 +681,7 @@ extern "C" int lk_sample(int device, int dtype, int64_t rows, int64_t vocab, con
     int bits = 0;  // 2^bits >= vocab
     while ((1ll << bits) < vocab) ++bits;
     SampleArgs a = {d_logits, ld, (int)vocab, 1, 0, 0, d_temperature, d_top_p, d_min_p, d_u, d_top_k,
-                    reinterpret_cast<long long *>(d_ids), d_probs, d_kept, (double)(1ull << (63 - bits))};
+                    reinterpret_cast<long long *>(d_ids), d_probs, d_kept, std::min(63 - bits, 50)};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == LK_F32) return sample_launch<float>(a, rows, device, st);
     if (dtype == LK_F16) return sample_launch<__half>(a, rows, device, st);
