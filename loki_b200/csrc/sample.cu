@@ -16,9 +16,9 @@
 //   pass gathers what reaches that bound in one CTA, and if that is 1,024 entries or fewer they are sorted there and
 //   all filters and the draw are settled among them.  Without a top-k the same happens when the bins that
 //   hold top_p of the weight have that few entries.
-// * Many.  A cut by count or weight: entries fall into 1,024 bins by the distance d = max - x, 32 bins to a
-//   factor of two (the bits of d without the low ones: monotone in x, and fine where a softmax has its
-//   weight).  The bin in which the measure reaches its target is cut again by the next bits of d, then by the
+// * Many.  A cut by count or weight: entries fall into 1,024 bins by the distance d = (max - x) / T, 128 bins to a
+//   factor of two from 1/8 to 32 (the bits of d without the low ones: monotone in x, and fine where a softmax
+//   has its weight; few entries of a warp meet in one bin).  The bin in which the measure reaches its target is cut again by the next bits of d, then by the
 //   bits of x, until at most 1,024 entries are left to be sorted, or all are equal and are cut by index.
 //   Then a pass sums the kept weights by warp and CTA, and the draw walks down those sums.
 #include "devops.cuh"
@@ -43,7 +43,7 @@ constexpr int ST = 1024, SWARPS = ST / 32;
 constexpr int SBINS = 1024;                // one thread per bin
 constexpr int SLIST = 1024;                // one thread per candidate
 constexpr int SMAX_CTAS = 16;
-constexpr int SD_SHIFT = 18, SD_BASE = (127 - 16) << 5;  // bins by d: exponent and 5 bits, from 2^-16 to 2^16
+constexpr int SD_SHIFT = 16, SD_BASE = (127 - 3) << 7;  // bins by d: exponent and 7 bits, from 2^-3 to 2^5
 using u64 = unsigned long long;
 
 struct alignas(16) SampleShared {
@@ -52,11 +52,11 @@ struct alignas(16) SampleShared {
     unsigned all_n[SBINS];
     u64 list[SLIST];                           // the first CTA's: candidates
     u64 sorted[SLIST];
-    double octave[32];                         // 2^(j/32)
+    double octave[64];                         // 2^(j/64)
     u64 warp_w[SWARPS];
     unsigned warp_n[SWARPS];
     u64 slot_w[SMAX_CTAS];                     // one word from every CTA of the row
-    unsigned slot_a[SMAX_CTAS], slot_b[SMAX_CTAS];
+    unsigned slot_top[SMAX_CTAS], slot_a[SMAX_CTAS], slot_b[SMAX_CTAS];
     unsigned listed;
     u64 cut;                                   // a decision of the first CTA, or of the one that holds an entry
     u64 found_w, found_before;
@@ -104,7 +104,9 @@ struct Row {
     const T *x;     // this CTA's stretch in global memory
     int rank, start, len, wlen, tid, lane, warp;
     float top;      // the largest score
-    double octaves; // 32 / (T ln 2): a distance in 32nds of an octave
+    double top_wide;
+    double octaves; // 64 / (T ln 2): a distance in 64ths of an octave
+    float per_t;    // 1 / T
     float least;    // min_p, and its logarithm
     double log_least;
     u64 thr;        // entries with a key at or above this are kept
@@ -128,32 +130,26 @@ struct Row {
     __device__ __forceinline__ bool kept(float v, int i) const { return v > thr_x || (v == thr_x && (unsigned)(start + i) <= thr_i); }
     __device__ __forceinline__ float entry(int i) const { return Elem<T>::get(i < a.cap ? data[i] : x[i]); }
 
-    // w * 2^F of a score, rounded.  Tang's scheme (ACM TOMS 15, 1989): with y = (x - max) / T / ln 2 * 32 = n + r, n whole,
-    // |r| <= 1/2:  w = 2^(n div 32) * 2^((n mod 32) / 32) * e^(r ln 2 / 32), the middle factor from a table, the last by its
-    // series to the fifth power (next term 2e-15).  The widening of x and both roundings to whole numbers are done by
-    // adding constants and on the bits: conversions issue at an eighth of the rate.
+    // w * 2^F of a score, rounded.  Tang's scheme (ACM TOMS 15, 1989): with y = (x - max) / T / ln 2 * 64 = n + r, n whole,
+    // |r| <= 1/2:  w = 2^(n div 64) * 2^((n mod 64) / 64) * e^(r ln 2 / 64), the middle factor from a table, the last by its
+    // series to the fourth power (next term 4e-14).  The roundings to whole numbers are done by adding constants, the power
+    // of two on the bits: conversions issue at an eighth of the rate.  No branches: the entries of a group overlap.
     __device__ __forceinline__ u64 weight(float v) const {
-        if (v == top) return 1ull << a.unit_bits;
-        if (!((v - top) * (float)octaves >= -32.0f * 64.0f)) return 0ull;  // below 2^-64 of the largest; an infinite distance too
-        const auto wide = [](float f) -> double {
-            const unsigned b = __float_as_uint(f);
-            if ((b & 0x7f800000u) == 0u) return (double)f;  // zero and subnormals
-            return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + (896u << 20))), (int)(b << 29));
-        };
         const double whole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number in the low word
-        const double dx = wide(v) - wide(top);
+        const double dx = (double)v - top_wide;
         const double t = fma(dx, octaves, whole);
+        const bool some = t >= whole - 64.0 * 64.0;  // else below 2^-64 of the largest; false for an infinite distance
         const double r = fma(dx, octaves, -(t - whole));
         const int n = __double2loint(t);
-        constexpr double c = 0.693147180559945309417232 / 32;
-        double q = fma(r, c * c * c * c * c / 120, c * c * c * c / 24);
-        q = fma(r, q, c * c * c / 6);
+        constexpr double c = 0.693147180559945309417232 / 64;
+        double q = fma(r, c * c * c * c / 24, c * c * c / 6);
         q = fma(r, q, c * c / 2);
         q = fma(r, q, c);
         q = fma(r, q, 1.0);
-        const double scale = __hiloint2double((1023 + (n >> 5) + a.unit_bits) << 20, 0);
-        const double w = fma(s.octave[n & 31] * q, scale, 4503599627370496.0);  // + 2^52; w <= 2^50
-        return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+        const double scale = __hiloint2double((1023 + (n >> 6) + a.unit_bits) << 20, 0);
+        const double w = fma(s.octave[n & 63] * q, scale, 4503599627370496.0);  // + 2^52; w <= 2^50
+        const u64 rounded = (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+        return v == top ? 1ull << a.unit_bits : (some ? rounded : 0ull);
     }
 
     // f(score, local index) for every entry of this warp's stretch; a stretch is whole groups but for the row's end
@@ -166,7 +162,18 @@ struct Row {
 #pragma unroll
             for (int e = 0; e < PER; ++e) f(Elem<T>::get(t[e]), i + e);
         }
-        for (int i = max(lo, a.cap) + lane; i < hi; i += 32) f(Elem<T>::get(x[i]), i);
+        int rest = max(lo, a.cap);  // on a group's boundary
+        if (rest < hi && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+            const int vecs = (hi - rest) / PER;
+            for (int g = lane; g < vecs; g += 32) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(x + rest + g * PER);
+                const T *t = reinterpret_cast<const T *>(&q);
+#pragma unroll
+                for (int e = 0; e < PER; ++e) f(Elem<T>::get(t[e]), rest + g * PER + e);
+            }
+            rest += vecs * PER;
+        }
+        for (int i = rest + lane; i < hi; i += 32) f(Elem<T>::get(x[i]), i);
     }
 
     // Sum of f over the row, by integers; warp_w keeps this CTA's warps' sums and slot_w the CTAs'.
@@ -240,17 +247,21 @@ struct Row {
     __device__ __forceinline__ u64 sort(u64 k, int n) const {
         int size_max = 32;
         while (size_max < n) size_max <<= 1;
+        const bool used = tid < size_max;  // whole warps
         for (int size = 2; size <= size_max; size <<= 1) {
             const bool down = (tid & size) == 0;  // this stretch descends
             for (int stride = size >> 1; stride > 0; stride >>= 1) {
                 u64 o;
                 if (stride >= 32) {
                     __syncthreads();
-                    s.sorted[tid] = k;
+                    if (used) s.sorted[tid] = k;
                     __syncthreads();
+                    if (!used) continue;
                     o = s.sorted[tid ^ stride];
-                } else
+                } else {
+                    if (!used) continue;
                     o = shfl_xor_u64(k, stride);
+                }
                 const bool low = (tid & stride) == 0;
                 if ((k < o) == (low == down)) k = o;
             }
@@ -300,26 +311,42 @@ struct Row {
     }
     // w >= min_p, as (x - max) / T >= log(min_p)
     __device__ __forceinline__ bool likely(float v) const {
-        return least <= 0.0f || v == top || ((double)v - (double)top) * (octaves * (0.693147180559945309417232 / 32)) >= log_least;
+        return least <= 0.0f || v == top || ((double)v - (double)top) * (octaves * (0.693147180559945309417232 / 64)) >= log_least;
     }
     static __device__ __forceinline__ u64 aim(float u, u64 total) {
         const double t = (double)u * (double)total;
         return t <= 0.0 ? 0ull : (t >= (double)total ? total - 1 : min((u64)t, total - 1));
     }
 
-    // Every CTA adds up its share of the row's bins and hands the sums to all.
+    // Every CTA adds up its share of the row's bins and hands the sums to all: thread (bin, CTA r) reads that bin of r's
+    // and, after the 2^g >= ctas threads of a bin have added up, writes the sum to r.
     template <bool MASS>
     __device__ __forceinline__ void join_bins() const {
+        if (a.ctas == 1) {
+            __syncthreads();
+            s.all_n[tid] = s.n[tid];
+            if (MASS) s.all_w[tid] = ((u64)s.hi[tid] << 32) + s.lo[tid];
+            __syncthreads();
+            return;
+        }
         sync();
-        const int share = (SBINS + a.ctas - 1) / a.ctas;
-        for (int b = rank * share + tid; b < min((rank + 1) * share, SBINS); b += ST) {
+        int wide = 2;
+        while (wide < a.ctas) wide <<= 1;
+        const int r = tid & (wide - 1), share = (SBINS + a.ctas - 1) / a.ctas, end = min((rank + 1) * share, SBINS);
+        for (int b0 = rank * share; b0 < end; b0 += ST / wide) {
+            const int b = b0 + tid / wide;
+            const bool there = b < end && r < a.ctas;
             unsigned n = 0;
             u64 w = 0;
-            for (int r = 0; r < a.ctas; ++r) {
-                n += s_get(s_at(&s.n[b], r));
-                if (MASS) w += ((u64)s_get(s_at(&s.hi[b], r)) << 32) + s_get(s_at(&s.lo[b], r));
+            if (there) {
+                n = s_get(s_at(&s.n[b], r));
+                if (MASS) w = ((u64)s_get(s_at(&s.hi[b], r)) << 32) + s_get(s_at(&s.lo[b], r));
             }
-            for (int r = 0; r < a.ctas; ++r) {
+            for (int d = 1; d < wide; d <<= 1) {
+                n += __shfl_xor_sync(0xffffffffu, n, d);
+                if (MASS) w += shfl_xor_u64(w, d);
+            }
+            if (there) {
                 s_put(s_at(&s.all_n[b], r), n);
                 if (MASS) s_put(s_at(&s.all_w[b], r), w);
             }
@@ -341,7 +368,7 @@ struct Row {
         __syncthreads();
         return s.found;
     }
-    __device__ __forceinline__ unsigned distance(float v) const { return __float_as_uint(v == top ? 0.0f : top - v); }
+    __device__ __forceinline__ unsigned distance(float v) const { return __float_as_uint(v == top ? 0.0f : (top - v) * per_t); }
     static __device__ __forceinline__ int first_bin(unsigned d) { return min(max((int)(d >> SD_SHIFT) - SD_BASE, 0), SBINS - 1); }
 
     // The candidates of bin b and above, in the first CTA's list: d below an end.  Their number (which may be more than fit).
@@ -349,7 +376,7 @@ struct Row {
         const unsigned end = (unsigned)(SD_BASE + b + 1) << SD_SHIFT;
         const float before = b >= SBINS - 1 ? CUDART_INF_F : __uint_as_float(end);
         each([&](float v, int i) {
-            if (top - v < before || v == top) {  // false for NaN and -infinity
+            if ((top - v) * per_t < before || v == top) {  // false for NaN and -infinity
                 const unsigned at = s_add(s_at(&s.listed, 0), 1u);
                 if (at < SLIST) s_put(s_at(&s.list[at], 0), key(v, i));
             }
@@ -429,7 +456,7 @@ struct Row {
             if (!by_image && sub > 0 && (level > 0 || (b > 0 && b < SBINS - 1))) {
                 in = sub;
                 pre = from + (unsigned)b;
-                sub = sub == SD_SHIFT ? 8 : 0;
+                sub = sub == SD_SHIFT ? SD_SHIFT - 10 : 0;
                 from = pre << (in - sub);
                 continue;
             }
@@ -505,7 +532,8 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     const float u = a.u[row];
     const bool bad = !(temp >= 0.0f) || p != p || least_in != least_in || u != u;
     if (temp == 0.0f) temp = 1.0f, k = 1;
-    if (warp == 1) s.octave[lane] = exp2(lane / 32.0);
+    if (tid < 64) s.octave[tid] = exp2(tid / 64.0);
+    if (a.ctas > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");  // waited for before the first write to another CTA
 
     // ---- the row comes in; its largest score ----
     const int held = min(w.len, a.cap);
@@ -538,14 +566,14 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     for (int i = held + tid; i < (int)round_up(held, PER); i += ST) w.data[i] = Elem<T>::put(CUDART_NAN_F);
     unsigned top = __reduce_max_sync(0xffffffffu, own);
     if (lane == 0) s.warp_n[warp] = top;
-    if (a.ctas > 1) w.sync();  // every CTA of the cluster runs before any writes to another
-    else __syncthreads();
+    __syncthreads();
+    if (a.ctas > 1) asm volatile("barrier.cluster.wait;" ::: "memory");  // every CTA of the cluster runs
     if (warp == 0) {
         top = __reduce_max_sync(0xffffffffu, s.warp_n[lane]);
-        if (lane < a.ctas) s_put(s_at(&s.slot_a[rank], lane), top);
+        if (lane < a.ctas) s_put(s_at(&s.slot_top[rank], lane), top);
     }
     w.sync();
-    for (int r = 0; r < a.ctas; ++r) top = max(top, s.slot_a[r]);
+    for (int r = 0; r < a.ctas; ++r) top = max(top, s.slot_top[r]);
     if (bad || top <= kNegInf) {  // the whole cluster agrees
         if (rank == 0 && tid == 0) {
             a.ids[row] = -1;
@@ -555,9 +583,10 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
         return;  // nothing is written to this CTA any more
     }
     w.top = f32_from_ord(top);
-    w.octaves = fmin(fmax(32.0 / (0.693147180559945309417232 * (double)temp), 1e-300), 1e300);  // an infinite distance stays one
+    w.top_wide = (double)w.top;
+    w.octaves = 64.0 / (0.693147180559945309417232 * (double)temp);
+    w.per_t = fminf(1.0f / temp, 3e38f);
     w.keep_from(make_key(kNegInf + 1, 0xffffffffu - 1u));
-    w.sync();  // the slots may be written again
 
     // ---- few candidates ----
     int n = 0;
