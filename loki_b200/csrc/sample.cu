@@ -21,6 +21,8 @@
 //   has its weight; few entries of a warp meet in one bin).  The bin in which the measure reaches its target is cut again by the next bits of d, then by the
 //   bits of x, until at most 1,024 entries are left to be sorted, or all are equal and are cut by index.
 //   Then a pass sums the kept weights by warp and CTA, and the draw walks down those sums.
+#include <cfloat>
+
 #include "devops.cuh"
 
 namespace lk {
@@ -45,19 +47,22 @@ constexpr int SLIST = 1024;                // one thread per candidate
 constexpr int SMAX_CTAS = 16;
 constexpr int SD_SHIFT = 16, SD_BASE = (127 - 3) << 7;  // bins by d: exponent and 7 bits, from 2^-3 to 2^5
 using u64 = unsigned long long;
+// Measured, 64 x 131,072 and 8 x 1,000,000 scores: a CTA's time per entry over all passes, for its start and its sorts, and what
+// the meetings of a cluster add.
+constexpr double SAMPLE_ENTRY_NS = 0.6, SAMPLE_CTA_NS = 10000.0, SAMPLE_MEET_NS = 5000.0;
 
 struct alignas(16) SampleShared {
     unsigned lo[SBINS], hi[SBINS], n[SBINS];   // this CTA's bins: weights (two words), entries
     u64 all_w[SBINS];                          // the row's bins
     unsigned all_n[SBINS];
-    u64 list[SLIST];                           // the first CTA's: candidates
-    u64 sorted[SLIST];
+    u64 list[SLIST];                           // this CTA's candidates
+    u64 sorted[SLIST];                         // scratch of the sort
     double octave[64];                         // 2^(j/64)
     u64 warp_w[SWARPS];
     unsigned warp_n[SWARPS];
     u64 slot_w[SMAX_CTAS];                     // one word from every CTA of the row
-    unsigned slot_top[SMAX_CTAS], slot_a[SMAX_CTAS], slot_b[SMAX_CTAS];
-    unsigned listed;
+    unsigned slot_top[SMAX_CTAS], slot_n[SMAX_CTAS], slot_a[SMAX_CTAS], slot_b[SMAX_CTAS];
+    unsigned noted;
     u64 cut;                                   // a decision of the first CTA, or of the one that holds an entry
     u64 found_w, found_before;
     int found;
@@ -75,10 +80,10 @@ __device__ __forceinline__ unsigned s_get(unsigned at) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
     return v;
 }
-__device__ __forceinline__ unsigned s_add(unsigned at, unsigned v) {
-    unsigned old;
-    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(at), "r"(v) : "memory");
-    return old;
+__device__ __forceinline__ u64 s_get64(unsigned at) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+    return v;
 }
 __device__ __forceinline__ u64 warp_sum(u64 v) {
 #pragma unroll
@@ -94,6 +99,51 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {  // inclusive
     return v;
 }
 
+// One step of a bitonic sort of one key per lane: this lane's stretch of 2 * STRIDE keys keeps the larger keys low (or high).
+template <int STRIDE>
+__device__ __forceinline__ void lane_step(u64 &k, bool down) {
+    const u64 o = shfl_xor_u64(k, STRIDE);
+    if ((k < o) == (((threadIdx.x & STRIDE) == 0) == down)) k = o;
+}
+// Keys sorted, largest first, one per thread (0 = none; n of them, in the first threads); every thread of the CTA takes part.
+// Strides below 32 by shuffles, wider ones through shared memory.
+__device__ __noinline__ u64 block_sort(SampleShared &s, u64 k, int n) {
+    const int tid = threadIdx.x;
+    int size_max = 32;
+    while (size_max < n) size_max <<= 1;
+    const bool used = tid < size_max;  // whole warps
+    if (used) {
+        lane_step<1>(k, (tid & 2) == 0);
+        lane_step<2>(k, (tid & 4) == 0), lane_step<1>(k, (tid & 4) == 0);
+        lane_step<4>(k, (tid & 8) == 0), lane_step<2>(k, (tid & 8) == 0), lane_step<1>(k, (tid & 8) == 0);
+        lane_step<8>(k, (tid & 16) == 0), lane_step<4>(k, (tid & 16) == 0), lane_step<2>(k, (tid & 16) == 0), lane_step<1>(k, (tid & 16) == 0);
+    }
+    for (int size = 32; size <= size_max; size <<= 1) {
+        const bool down = (tid & size) == 0;  // this stretch descends
+        for (int stride = size >> 1; stride >= 32; stride >>= 1) {
+            __syncthreads();
+            if (used) s.sorted[tid] = k;
+            __syncthreads();
+            if (used) {
+                const u64 o = s.sorted[tid ^ stride];
+                if ((k < o) == (((tid & stride) == 0) == down)) k = o;
+            }
+        }
+        if (used) lane_step<16>(k, down), lane_step<8>(k, down), lane_step<4>(k, down), lane_step<2>(k, down), lane_step<1>(k, down);
+    }
+    return k;
+}
+// Inclusive running sum over the threads of the CTA.
+__device__ __noinline__ u64 block_scan(SampleShared &s, u64 v) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    v = warp_scan(v, lane);
+    __syncthreads();
+    if (lane == 31) s.warp_w[warp] = v;
+    __syncthreads();
+    const u64 other = warp_scan(s.warp_w[lane], lane);
+    return warp == 0 ? v : v + __shfl_sync(0xffffffffu, other, warp - 1);
+}
+
 // One row, as the CTAs of its cluster see it.
 template <typename T>
 struct Row {
@@ -104,11 +154,12 @@ struct Row {
     const T *x;     // this CTA's stretch in global memory
     int rank, start, len, wlen, tid, lane, warp;
     float top;      // the largest score
+    float bottom;   // a score so far below it that it weighs nothing
+    bool alone;     // nothing else weighs: it is +infinity, or T is that small
     double top_wide;
     double octaves; // 64 / (T ln 2): a distance in 64ths of an octave
-    float per_t;    // 1 / T
-    float least;    // min_p, and its logarithm
-    double log_least;
+    float temp, per_t;  // T, 1 / T
+    u64 floor;      // min_p: the lowest key that it keeps
     u64 thr;        // entries with a key at or above this are kept
     float thr_x;    // its score and its index
     unsigned thr_i;
@@ -130,15 +181,14 @@ struct Row {
     __device__ __forceinline__ bool kept(float v, int i) const { return v > thr_x || (v == thr_x && (unsigned)(start + i) <= thr_i); }
     __device__ __forceinline__ float entry(int i) const { return Elem<T>::get(i < a.cap ? data[i] : x[i]); }
 
-    // w * 2^F of a score, rounded.  Tang's scheme (ACM TOMS 15, 1989): with y = (x - max) / T / ln 2 * 64 = n + r, n whole,
-    // |r| <= 1/2:  w = 2^(n div 64) * 2^((n mod 64) / 64) * e^(r ln 2 / 64), the middle factor from a table, the last by its
-    // series to the fourth power (next term 4e-14).  The roundings to whole numbers are done by adding constants, the power
-    // of two on the bits: conversions issue at an eighth of the rate.  No branches: the entries of a group overlap.
+    // w * 2^F of a score, rounded, where others than the largest weigh.  Tang's scheme (ACM TOMS 15, 1989): with y =
+    // (x - max) / T / ln 2 * 64 = n + r, n whole, |r| <= 1/2:  w = 2^(n div 64) * 2^((n mod 64) / 64) * e^(r ln 2 / 64), the
+    // middle factor from a table, the last by its series to the fourth power (next term 4e-14).  The roundings to whole
+    // numbers are done by adding constants, the power of two on the bits: conversions issue at an eighth of the rate.
     __device__ __forceinline__ u64 weight(float v) const {
         const double whole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number in the low word
-        const double dx = (double)v - top_wide;
+        const double dx = (double)fmaxf(v, bottom) - top_wide;
         const double t = fma(dx, octaves, whole);
-        const bool some = t >= whole - 64.0 * 64.0;  // else below 2^-64 of the largest; false for an infinite distance
         const double r = fma(dx, octaves, -(t - whole));
         const int n = __double2loint(t);
         constexpr double c = 0.693147180559945309417232 / 64;
@@ -146,41 +196,68 @@ struct Row {
         q = fma(r, q, c * c / 2);
         q = fma(r, q, c);
         q = fma(r, q, 1.0);
-        const double scale = __hiloint2double((1023 + (n >> 6) + a.unit_bits) << 20, 0);
+        const double scale = __hiloint2double(((n & ~63) << 14) + ((1023 + a.unit_bits) << 20), 0);
         const double w = fma(s.octave[n & 63] * q, scale, 4503599627370496.0);  // + 2^52; w <= 2^50
-        const u64 rounded = (u64)__double_as_longlong(w) & 0xfffffffffffffull;
-        return v == top ? 1ull << a.unit_bits : (some ? rounded : 0ull);
+        return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ u64 weight_of(float v) const {
+        if (alone) return v == top ? 1ull << a.unit_bits : 0ull;
+        return weight(v);
+    }
+    // Of four scores; those that are not kept weigh nothing.
+    __device__ __forceinline__ void weights(const float (&v)[4], const bool (&k)[4], u64 (&w)[4]) const {
+        if (alone) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = k[e] && v[e] == top ? 1ull << a.unit_bits : 0ull;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const u64 m = weight(v[e]);
+                w[e] = k[e] ? m : 0ull;
+            }
+        }
     }
 
-    // f(score, local index) for every entry of this warp's stretch; a stretch is whole groups but for the row's end
+    // f(four scores, local index of the first) for the entries of this warp's stretch, NaN for those past its end.  Four
+    // at a time, because their weights are then computed side by side; one copy of f in the code, because a kernel this
+    // short waits for its instructions.
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
-        const int lo = warp * wlen, hi = min(lo + wlen, len), held = min(hi, a.cap);
-        for (int i = lo + lane * PER; i < held; i += 32 * PER) {
-            const uint4 q = *reinterpret_cast<const uint4 *>(data + i);
-            const T *t = reinterpret_cast<const T *>(&q);
+        const int lo = warp * wlen, hi = min(lo + wlen, len);
+#pragma unroll 1
+        for (int i = lo + lane * 4; i < hi; i += 128) {
+            float v[4];
+            if (i < a.cap) {  // whole: the stretch is padded with NaN
+                if constexpr (sizeof(T) == 4) {
+                    const float4 q = *reinterpret_cast<const float4 *>(data + i);
+                    v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+                } else {
+                    const uint2 q = *reinterpret_cast<const uint2 *>(data + i);
+                    const T *t = reinterpret_cast<const T *>(&q);
+                    v[0] = Elem<T>::get(t[0]), v[1] = Elem<T>::get(t[1]), v[2] = Elem<T>::get(t[2]), v[3] = Elem<T>::get(t[3]);
+                }
+            } else {
 #pragma unroll
-            for (int e = 0; e < PER; ++e) f(Elem<T>::get(t[e]), i + e);
-        }
-        int rest = max(lo, a.cap);  // on a group's boundary
-        if (rest < hi && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-            const int vecs = (hi - rest) / PER;
-            for (int g = lane; g < vecs; g += 32) {
-                const uint4 q = *reinterpret_cast<const uint4 *>(x + rest + g * PER);
-                const T *t = reinterpret_cast<const T *>(&q);
-#pragma unroll
-                for (int e = 0; e < PER; ++e) f(Elem<T>::get(t[e]), rest + g * PER + e);
+                for (int e = 0; e < 4; ++e) v[e] = i + e < hi ? Elem<T>::get(x[i + e]) : CUDART_NAN_F;
             }
-            rest += vecs * PER;
+            f(v, i);
         }
-        for (int i = rest + lane; i < hi; i += 32) f(Elem<T>::get(x[i]), i);
     }
 
-    // Sum of f over the row, by integers; warp_w keeps this CTA's warps' sums and slot_w the CTAs'.
-    template <typename F>
-    __device__ __forceinline__ u64 sums(F f) const {
+    // Sum over the entries with keep(score, index) of their weights (MASS) or their number; warp_w keeps this CTA's warps'
+    // sums and slot_w the CTAs'.
+    template <bool MASS, typename K>
+    __device__ __forceinline__ u64 sums(K keep) const {
         u64 w = 0;
-        each([&](float v, int i) { w += f(v, i); });
+        each([&](const float (&v)[4], int i) {
+            bool k[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = keep(v[e], i + e);
+            if (!(k[0] | k[1] | k[2] | k[3])) return;
+            u64 m[4] = {k[0], k[1], k[2], k[3]};
+            if (MASS) weights(v, k, m);
+            w += (m[0] + m[1]) + (m[2] + m[3]);
+        });
         w = warp_sum(w);
         __syncthreads();
         if (lane == 0) s.warp_w[warp] = w;
@@ -194,11 +271,12 @@ struct Row {
         for (int r = 0; r < a.ctas; ++r) all += s.slot_w[r];
         return all;
     }
-    // The entry at which the running sum of f (in the order of the indexes) first exceeds `target`, which
-    // is below the sum that sums(f) has just returned: the CTA that holds it sets found (local index) and
-    // found_w (its f); in the others found is -1.  No meeting of the cluster.
-    template <typename F>
-    __device__ __forceinline__ void walk(F f, u64 target) const {
+    // The entry at which the running sum (in the order of the indexes) first exceeds `target`, which is below the sum
+    // that sums() has just returned for the same entries: the CTA that holds it sets found (local index) and found_w (its
+    // measure); in the others found is -1.  No meeting of the cluster.
+    template <bool MASS, typename K>
+    __device__ __forceinline__ void walk(K keep, u64 target) const {
+        const auto f = [&](float v, int i) -> u64 { return keep(v, i) ? (MASS ? weight_of(v) : 1ull) : 0ull; };
         __syncthreads();
         if (tid == 0) s.found = -1;
         u64 before = 0;
@@ -242,66 +320,30 @@ struct Row {
         __syncthreads();
     }
 
-    // Keys sorted, largest first, one per thread (0 = none); every thread of the CTA takes part.  Strides below 32 by
-    // shuffles, wider ones through shared memory.
-    __device__ __forceinline__ u64 sort(u64 k, int n) const {
-        int size_max = 32;
-        while (size_max < n) size_max <<= 1;
-        const bool used = tid < size_max;  // whole warps
-        for (int size = 2; size <= size_max; size <<= 1) {
-            const bool down = (tid & size) == 0;  // this stretch descends
-            for (int stride = size >> 1; stride > 0; stride >>= 1) {
-                u64 o;
-                if (stride >= 32) {
-                    __syncthreads();
-                    if (used) s.sorted[tid] = k;
-                    __syncthreads();
-                    if (!used) continue;
-                    o = s.sorted[tid ^ stride];
-                } else {
-                    if (!used) continue;
-                    o = shfl_xor_u64(k, stride);
-                }
-                const bool low = (tid & stride) == 0;
-                if ((k < o) == (low == down)) k = o;
-            }
-        }
-        return k;
-    }
-    // Inclusive running sum over the threads of the CTA.
-    __device__ __forceinline__ u64 block_scan(u64 v) const {
-        v = warp_scan(v, lane);
-        __syncthreads();
-        if (lane == 31) s.warp_w[warp] = v;
-        __syncthreads();
-        const u64 other = warp_scan(s.warp_w[lane], lane);
-        return warp == 0 ? v : v + __shfl_sync(0xffffffffu, other, warp - 1);
-    }
-
-    // The first CTA has every entry that may be kept in its list (n of them): all filters, and the draw.  `all`: the weight
+    // The lists hold every entry that may be kept (n of them): in the first CTA, all filters and the draw.  `all`: the weight
     // that top_p refers to, 0 = that of the k first.
     __device__ void finish(long long row, int n, int k, float p, float u, u64 all) const {
-        const u64 mine = sort(tid < n ? s.list[tid] : 0ull, n);  // thread t holds the entry of rank t
+        const u64 mine = block_sort(s, fetch(), n);  // thread t holds the entry of rank t
         const float v = f32_from_ord(key_ord(mine));
         const bool in = tid < n && (k <= 0 || tid < k);
-        const u64 w = in ? weight(v) : 0ull;
-        const u64 inc = block_scan(w);
+        const u64 w = in ? weight_of(v) : 0ull;
+        const u64 inc = block_scan(s, w);
         if (tid == ST - 1) s.found_before = inc;
         __syncthreads();
         if (all == 0) all = s.found_before;
         const u64 want = p < 1.0f ? (p <= 0.0f ? 1ull : max((u64)ceil((double)p * (double)all), (u64)1)) : ~0ull;
-        const bool keep = in && inc - w < want && (tid == 0 || likely(v));
+        const bool keep = in && inc - w < want && (tid == 0 || mine >= floor);
         const int count = __syncthreads_count(keep);
         if (tid == count - 1) s.found_w = inc;
         s.all_w[tid] = w;
         const unsigned slot = key_slot(mine);
         // the kept ones by index: largest first of ~(index, rank)
-        const u64 by_index = sort(keep ? ~(((u64)slot << 10) | (unsigned)tid) : 0ull, count);
+        const u64 by_index = block_sort(s, keep ? ~(((u64)slot << 10) | (unsigned)tid) : 0ull, count);
         __syncthreads();
         const u64 total = s.found_w;
         const unsigned from = (unsigned)~by_index & 1023u;
         const u64 w2 = tid < count ? s.all_w[from] : 0ull;
-        const u64 run = block_scan(w2);
+        const u64 run = block_scan(s, w2);
         const u64 target = aim(u, total);
         if (run - w2 <= target && target < run) {
             a.ids[row] = (long long)((~by_index) >> 10);
@@ -309,9 +351,17 @@ struct Row {
             if (a.kept) a.kept[row] = count;
         }
     }
-    // w >= min_p, as (x - max) / T >= log(min_p)
-    __device__ __forceinline__ bool likely(float v) const {
-        return least <= 0.0f || v == top || ((double)v - (double)top) * (octaves * (0.693147180559945309417232 / 64)) >= log_least;
+    // The lowest key with w >= min_p, i.e. (x - max) / T >= log(min_p): by bisection over the images.
+    __device__ __forceinline__ u64 lowest(float min_p) const {
+        if (min_p <= 0.0f) return 0ull;
+        const double end = log((double)min_p);
+        unsigned lo = kNegInf + 1, hi = ord_from_f32(top);  // the largest score is always kept
+        while (lo < hi) {
+            const unsigned mid = lo + (hi - lo) / 2;
+            if (((double)f32_from_ord(mid) - top_wide) * (octaves * (0.693147180559945309417232 / 64)) >= end) hi = mid;
+            else lo = mid + 1;
+        }
+        return make_key(lo, ~0u);
     }
     static __device__ __forceinline__ u64 aim(float u, u64 total) {
         const double t = (double)u * (double)total;
@@ -357,13 +407,13 @@ struct Row {
     __device__ __forceinline__ void clear_bins() const {
         s.n[tid] = 0;
         if (MASS) s.lo[tid] = s.hi[tid] = 0;
-        if (tid == 0) s.listed = 0;
+        if (tid == 0) s.noted = 0;
         __syncthreads();
     }
     // The bin in which the running measure (from `base` on) reaches `want`, -1 if none; found_before = what lies above it.
     __device__ __forceinline__ int reach(u64 m, u64 base, u64 want) const {
         if (tid == 0) s.found = -1;
-        const u64 inc = block_scan(m) + base;
+        const u64 inc = block_scan(s, m) + base;
         if (inc >= want && inc - m < want) s.found = tid, s.found_before = inc - m;
         __syncthreads();
         return s.found;
@@ -371,23 +421,54 @@ struct Row {
     __device__ __forceinline__ unsigned distance(float v) const { return __float_as_uint(v == top ? 0.0f : (top - v) * per_t); }
     static __device__ __forceinline__ int first_bin(unsigned d) { return min(max((int)(d >> SD_SHIFT) - SD_BASE, 0), SBINS - 1); }
 
-    // The candidates of bin b and above, in the first CTA's list: d below an end.  Their number (which may be more than fit).
+    // The candidates of bin b and above, in the lists: d below an end.  Their number (which may be more than fit).
     __device__ __forceinline__ unsigned gather_to(int b) const {
         const unsigned end = (unsigned)(SD_BASE + b + 1) << SD_SHIFT;
         const float before = b >= SBINS - 1 ? CUDART_INF_F : __uint_as_float(end);
-        each([&](float v, int i) {
-            if ((top - v) * per_t < before || v == top) {  // false for NaN and -infinity
-                const unsigned at = s_add(s_at(&s.listed, 0), 1u);
-                if (at < SLIST) s_put(s_at(&s.list[at], 0), key(v, i));
-            }
+        // a score below all candidates, for a quick look: the end of the bins with room for the roundings
+        const double reach_d = (double)before * (double)temp;
+        float near = (float)(top_wide - reach_d - 1e-5 * (reach_d + fabs(top_wide)) - 1e-37);
+        if (!(near < CUDART_INF_F)) near = -CUDART_INF_F;
+        each([&](const float (&v)[4], int i) {
+            if (!(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= near)) return;  // fmaxf passes over NaN
+            bool in[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) in[e] = (top - v[e]) * per_t < before || v[e] == top;  // false for NaN and -infinity
+            note(in, v, i);
         });
+        return deliver();
+    }
+    // Candidates go to this CTA's own list; deliver() tells all CTAs how many there are (more than SLIST: some are missing),
+    // and the first CTA fetches the lists: thread t has candidate t.
+    __device__ __forceinline__ void note(const bool (&in)[4], const float (&v)[4], int i) const {
+        if (!(in[0] | in[1] | in[2] | in[3])) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (in[e]) {
+                const unsigned at = atomicAdd(&s.noted, 1u);
+                if (at < SLIST) s.list[at] = key(v[e], i + e);
+            }
+    }
+    __device__ __forceinline__ unsigned deliver() const {
+        __syncthreads();
+        if (tid < a.ctas) s_put(s_at(&s.slot_n[rank], tid), s.noted);
         sync();
-        return s_get(s_at(&s.listed, 0));
+        unsigned n = 0;
+        for (int r = 0; r < a.ctas; ++r) n += s.slot_n[r];
+        return n;
+    }
+    __device__ __forceinline__ u64 fetch() const {
+        unsigned at = tid;
+        for (int r = 0; r < a.ctas; ++r) {
+            if (at < s.slot_n[r]) return s_get64(s_at(&s.list[at], r));
+            at -= s.slot_n[r];
+        }
+        return 0ull;
     }
 
     // MASS: moves thr up to the last entry of the shortest prefix that holds the share p of the kept weight.
-    // Else: to the k-th entry.  Returns the number of candidates when all that may be kept is in the first
-    // CTA's list instead (`whole`: thr is still at the row's end), with the row's weight in *all; 0 when thr has been moved.
+    // Else: to the k-th entry.  Returns the number of candidates when all that may be kept is in the
+    // lists instead (`whole`: thr is still at the row's end), with the row's weight in *all; 0 when thr has been moved.
     template <bool MASS>
     __device__ int cut(int k, float p, bool whole, u64 *all) {
         u64 want = (u64)k, base = 0;  // base: measure of what lies above the current bin
@@ -405,22 +486,28 @@ struct Row {
                 const unsigned d = distance(v);
                 return (d >> in) == pre ? min(max((int)(d >> sub) - (int)from, 0), SBINS - 1) : -1;
             };
-            each([&](float v, int i) {
-                if (!kept(v, i)) return;
-                const int b = bin(v);
-                if (b < 0) return;
-                atomicAdd(&s.n[b], 1u);
-                if (MASS) {
-                    const u64 w = weight(v);
-                    const unsigned l = (unsigned)w, old = atomicAdd(&s.lo[b], l);
-                    const unsigned h = (unsigned)(w >> 32) + (old + l < l ? 1u : 0u);
-                    if (h) atomicAdd(&s.hi[b], h);
-                }
+            each([&](const float (&v)[4], int i) {
+                int at[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) at[e] = kept(v[e], i + e) ? bin(v[e]) : -1;
+                if ((at[0] & at[1] & at[2] & at[3]) < 0) return;  // none of the four: all are -1
+                u64 w[4];
+                if (MASS) weights(v, {at[0] >= 0, at[1] >= 0, at[2] >= 0, at[3] >= 0}, w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (at[e] >= 0) {
+                        atomicAdd(&s.n[at[e]], 1u);
+                        if (MASS) {
+                            const unsigned l = (unsigned)w[e], old = atomicAdd(&s.lo[at[e]], l);
+                            const unsigned h = (unsigned)(w[e] >> 32) + (old + l < l ? 1u : 0u);
+                            if (h) atomicAdd(&s.hi[at[e]], h);
+                        }
+                    }
             });
             join_bins<MASS>();
             const u64 m = MASS ? s.all_w[tid] : (u64)s.all_n[tid];
             if (MASS && level == 0) {
-                const u64 inc = block_scan(m);
+                const u64 inc = block_scan(s, m);
                 if (tid == ST - 1) s.cut = inc;
                 __syncthreads();
                 *all = s.cut;
@@ -431,20 +518,23 @@ struct Row {
             base = s.found_before;
             const unsigned n = s.all_n[b];
             if (level == 0 && whole) {  // everything down to this bin
-                const u64 upto = block_scan(tid <= b ? s.all_n[tid] : 0u);
+                const u64 upto = block_scan(s, tid <= b ? s.all_n[tid] : 0u);
                 if (tid == ST - 1) s.found_w = upto;
                 __syncthreads();
                 if (s.found_w <= SLIST && b < SBINS - 1) return (int)gather_to(b);
             }
             if (n <= SLIST) {
-                each([&](float v, int i) {
-                    if (kept(v, i) && bin(v) == b) s_put(s_at(&s.list[s_add(s_at(&s.listed, 0), 1u)], 0), key(v, i));
+                each([&](const float (&v)[4], int i) {
+                    bool among[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) among[e] = kept(v[e], i + e) && bin(v[e]) == b;
+                    note(among, v, i);
                 });
-                sync();
+                deliver();
                 if (rank == 0) {
-                    const u64 mine = sort(tid < (int)n ? s.list[tid] : 0ull, (int)n);
-                    const u64 w = tid >= (int)n ? 0ull : (MASS ? weight(f32_from_ord(key_ord(mine))) : 1ull);
-                    const u64 inc = block_scan(w) + base;
+                    const u64 mine = block_sort(s, fetch(), (int)n);
+                    const u64 w = tid >= (int)n ? 0ull : (MASS ? weight_of(f32_from_ord(key_ord(mine))) : 1ull);
+                    const u64 inc = block_scan(s, w) + base;
                     if (inc >= want && inc - w < want)
                         for (int r = 0; r < a.ctas; ++r) s_put(s_at(&s.cut, r), mine);
                 }
@@ -462,11 +552,13 @@ struct Row {
             }
             // the bits of the scores, between the least and the largest of the bin
             unsigned least = ~0u, most = 0;
-            each([&](float v, int i) {
-                if (kept(v, i) && bin(v) == b) {
-                    const unsigned o = ord_from_f32(v);
-                    least = min(least, o), most = max(most, o);
-                }
+            each([&](const float (&v)[4], int i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (kept(v[e], i + e) && bin(v[e]) == b) {
+                        const unsigned o = ord_from_f32(v[e]);
+                        least = min(least, o), most = max(most, o);
+                    }
             });
             least = __reduce_min_sync(0xffffffffu, least);
             most = __reduce_max_sync(0xffffffffu, most);
@@ -487,12 +579,12 @@ struct Row {
             sync();  // the slots may be written again
             if (olo == ohi) {  // equal scores: the first of them, by index
                 const float tied = f32_from_ord(olo);
-                const u64 each_w = MASS ? weight(tied) : 1ull;
+                const u64 each_w = MASS ? weight_of(tied) : 1ull;
                 const u64 need = (want - base + each_w - 1) / each_w;  // each_w > 0: the bin reaches the target
                 if (need < n) {
-                    const auto tie = [&](float v, int i) -> u64 { return v == tied && kept(v, i); };
-                    sums(tie);
-                    walk(tie, need - 1);
+                    const auto tie = [&](float v, int i) { return v == tied && kept(v, i); };
+                    sums<false>(tie);
+                    walk<false>(tie, need - 1);
                     if (tid == 0 && s.found >= 0)
                         for (int r = 0; r < a.ctas; ++r) s_put(s_at(&s.cut, r), key(tied, s.found));
                     sync();
@@ -527,8 +619,6 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     int k = a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f;
     const float least_in = a.min_p ? a.min_p[row] : 0.0f;
-    w.least = fminf(least_in, 1.0f);  // the first is always kept
-    w.log_least = w.least > 0.0f ? log((double)w.least) : 0.0;
     const float u = a.u[row];
     const bool bad = !(temp >= 0.0f) || p != p || least_in != least_in || u != u;
     if (temp == 0.0f) temp = 1.0f, k = 1;
@@ -584,8 +674,15 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     }
     w.top = f32_from_ord(top);
     w.top_wide = (double)w.top;
+    w.temp = temp;
     w.octaves = 64.0 / (0.693147180559945309417232 * (double)temp);
     w.per_t = fminf(1.0f / temp, 3e38f);
+    // 62 octaves down a weight rounds to 0 (F <= 50).  Where the next lower float32 is further down than that, nothing but the
+    // largest score weighs; else `bottom` is 62 to 124 octaves down, or the lowest score there is.
+    const double deep = 62.0 * 0.693147180559945309417232 * (double)temp;
+    w.alone = !(w.top_wide - (double)nextafterf(w.top, -CUDART_INF_F) < deep);  // true for +infinity
+    w.bottom = __double2float_rd(fmax(w.top_wide - deep, -(double)FLT_MAX));
+    w.floor = w.lowest(least_in);
     w.keep_from(make_key(kNegInf + 1, 0xffffffffu - 1u));
 
     // ---- few candidates ----
@@ -598,7 +695,6 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
         const int b = w.reach(s.all_n[tid], 0, (u64)k);
         if (b >= 0 && b < SBINS - 1) n = (int)w.gather_to(b);
         if (n > SLIST) n = 0;
-        w.sync();  // the count has been read
     }
     // ---- the cuts ----
     if (n == 0) {
@@ -614,15 +710,16 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
 
     // ---- the draw ----
     unsigned count = 0;
-    const auto kept_weight = [&](float v, int i) -> u64 {
-        if (!w.kept(v, i) || !w.likely(v)) return 0ull;
-        ++count;
-        return w.weight(v);
+    const auto keep = [&](float v, int i) {
+        const bool yes = w.kept(v, i);
+        count += yes;
+        return yes;
     };
-    all = w.sums(kept_weight);
+    w.keep_from(max(w.thr, w.floor));
+    all = w.template sums<true>(keep);
     count = __reduce_add_sync(0xffffffffu, count);
     if (lane == 0) s.warp_n[warp] = count;
-    w.walk(kept_weight, Row<T>::aim(u, all));
+    w.template walk<true>(keep, Row<T>::aim(u, all));
     __syncthreads();
     if (s.found >= 0 && tid == 0) {
         a.ids[row] = start + s.found;
@@ -646,44 +743,43 @@ template <typename T>
 static int sample_launch(SampleArgs a, long long rows, int device, cudaStream_t st) {
     constexpr size_t kSmem = 227 * 1024;
     constexpr int kHold = (int)((kSmem - sizeof(SampleShared)) / sizeof(T)) & ~63;
-    static bool sized[kMaxDevices];
-    static int most[kMaxDevices];  // CTAs of a row
-    if (!sized[device]) {
-        LK_CUDA(cudaFuncSetAttribute((const void *)k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
-        LK_CUDA(cudaFuncSetAttribute((const void *)k_sample<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        cudaLaunchConfig_t all = {};  // does a cluster of 16 full CTAs fit on this GPU?
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)(most[device] = SMAX_CTAS);
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        all.gridDim = dim3(SMAX_CTAS);
-        all.blockDim = dim3(ST);
-        all.dynamicSmemBytes = kSmem;
-        all.attrs = attr;
-        all.numAttrs = 1;
-        int fit = 0;
-        if (cudaOccupancyMaxActiveClusters(&fit, k_sample<T>, &all) != cudaSuccess || fit < 1) most[device] = 8;  // the portable size
-        cudaGetLastError();
-        sized[device] = true;
-    }
-    // as many CTAs to a row as its entries want (4,096 or more each) while the GPU has room for all rows at once, and at
-    // least as many as hold the row
-    const int sms = sm_count(device);
-    a.ctas = 1;
-    while (a.ctas < most[device] && (a.vocab > (long long)kHold * a.ctas || (a.vocab >= 8192 * a.ctas && rows * a.ctas * 2 <= sms))) a.ctas *= 2;
-    a.seg = (int)round_up((a.vocab + a.ctas - 1) / a.ctas, 64);
-    a.cap = std::min(a.seg, kHold);
+    static bool asked[kMaxDevices];
+    static int fit[kMaxDevices][SMAX_CTAS + 1];  // clusters of so many full CTAs that run at the same time
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * a.ctas));
-    cfg.blockDim = dim3(ST);
-    cfg.dynamicSmemBytes = sizeof(SampleShared) + (size_t)a.cap * sizeof(T);
-    cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)a.ctas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(ST);
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if (!asked[device]) {
+        LK_CUDA(cudaFuncSetAttribute((const void *)k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+        LK_CUDA(cudaFuncSetAttribute((const void *)k_sample<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        cfg.dynamicSmemBytes = kSmem;
+        for (int c = 1; c <= SMAX_CTAS; ++c) {
+            attr[0].val.clusterDim.x = (unsigned)c;
+            cfg.gridDim = dim3((unsigned)c);
+            if (cudaOccupancyMaxActiveClusters(&fit[device][c], k_sample<T>, &cfg) != cudaSuccess) fit[device][c] = 0;
+        }
+        cudaGetLastError();
+        asked[device] = true;
+    }
+    // The number of CTAs to a row that finishes first: clusters run in waves, a CTA's time is its entries (those past what
+    // its shared memory holds cost more) and its meetings.
+    double least = 1e300;
+    for (int c = 1; c <= SMAX_CTAS; ++c) {
+        if (c > 1 && fit[device][c] < 1) continue;
+        const double waves = (double)((rows + std::max(fit[device][c], 1) - 1) / std::max(fit[device][c], 1));
+        const double seg = (double)((a.vocab + c - 1) / c);
+        const double cost = waves * (SAMPLE_ENTRY_NS * seg + SAMPLE_ENTRY_NS * 0.5 * std::max(0.0, seg - kHold) + (c > 1 ? SAMPLE_MEET_NS : 0.0) + SAMPLE_CTA_NS);
+        if (cost < least) least = cost, a.ctas = c;
+    }
+    a.seg = (int)round_up((a.vocab + a.ctas - 1) / a.ctas, 64);
+    a.cap = std::min(a.seg, kHold);
+    attr[0].val.clusterDim.x = (unsigned)a.ctas;
+    cfg.gridDim = dim3((unsigned)(rows * a.ctas));
+    cfg.dynamicSmemBytes = sizeof(SampleShared) + (size_t)a.cap * sizeof(T);
+    cfg.stream = st;
     return launch_cfg("lk_sample", k_sample<T>, cfg, a);
 }
 
