@@ -124,6 +124,8 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
     const int s0 = (int)((long long)g.slices * part_of / (PAIR ? 1 : g.split));
     const int s1 = (int)((long long)g.slices * (part_of + 1) / (PAIR ? 1 : g.split));
 
+    const int early = PAIR ? 0 : min(g.stages, s1 - s0);  // slices of the first tile that need no free stage waited for
+
     if (tid == 0) {
         for (int i = 0; i < g.stages; ++i) {
             g_mbar_init(&ctl->full[i], 1);
@@ -135,6 +137,14 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
         }
         ctl->failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (!PAIR && first < g.tiles) {  // the first stages are on their way while the CTA sets itself up
+            const int yw = (int)(first / g.tiles_m) * LW, ya = (int)(first % g.tiles_m) * g.mt;
+            for (int i = 0; i < early; ++i) {
+                g_mbar_expect_tx(&ctl->full[i], (unsigned)(LW_BYTES + a_bytes));
+                l_load<PAIR>(g_smem(sm_w + (size_t)i * LW_BYTES), &tm_w, (s0 + i) * LSLICE, yw, g_smem(&ctl->full[i]));
+                l_load<PAIR>(g_smem(sm_a + (size_t)i * a_bytes), &tm_a, (s0 + i) * LSLICE, ya, g_smem(&ctl->full[i]));
+            }
+        }
     }
     if (warp == 1) {
         __syncwarp();
@@ -164,7 +174,7 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
             for (int s = s0; s < s1; ++s) {
                 ok = g_mbar_wait_warp(&ctl->empty[stage], phase ^ 1u, failed);
                 if (!ok) break;
-                if (g_elect_one()) {
+                if (!(t == first && s - s0 < early) && g_elect_one()) {
                     const unsigned bar = PAIR ? g_leader_addr(g_smem(&ctl->full[stage])) : g_smem(&ctl->full[stage]);
                     if (cta_of == 0) g_mbar_expect_tx(&ctl->full[stage], (unsigned)(CG * (LW_BYTES + a_bytes)));
                     l_load<PAIR>(g_smem(sm_w + (size_t)stage * LW_BYTES), &tm_w, s * LSLICE, yw, bar);
@@ -302,29 +312,57 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (!PAIR && g.split > 1) {  // one tile per cluster
-        g_pair_sync();
         const long long j0 = (first / g.tiles_m) * LW, i0 = (first % g.tiles_m) * g.mt;
-        const int lo = g.mt * part_of / g.split, hi = g.mt * (part_of + 1) / g.split;
+        const int lo = g.mt * part_of / g.split * LW, hi = g.mt * (part_of + 1) / g.split * LW;
         const unsigned base = g_smem(smem);
-        for (int e = lo * LW + tid; e < hi * LW; e += LTHREADS) {
+        // what the epilogue needs is on its way while the cluster meets; LTHREADS is a multiple of neither, so each value
+        // has a thread of its own
+        constexpr int V = 4;
+        const auto inputs = [&](int e, float &s, float &b, float &r) {
             const long long i = i0 + e / LW, j = j0 + e % LW;
-            if (i >= p.m || j >= p.n) continue;
-            float x;
-            int whole = 0;
-            float sum = 0.0f;
-            for (int r = 0; r < g.split; ++r) {
-                unsigned at, bits;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + (unsigned)e * 4u), "r"(r));
-                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(bits) : "r"(at) : "memory");
-                if constexpr (I8) whole += (int)bits;
-                else sum += __uint_as_float(bits);
+            s = 1.0f, b = r = 0.0f;
+            if (e < hi && i < p.m && j < p.n) {
+                s = scale_of(p.a_scales, i) * scale_of(p.w_scales, j);
+                if (p.bias != nullptr) b = Elem<Out>::get(static_cast<const Out *>(p.bias)[j]);
+                if (p.residual != nullptr) r = Elem<Out>::get(static_cast<const Out *>(p.residual)[i * p.ldr + j]);
             }
-            x = I8 ? (float)whole : sum;
-            float y[1] = {x * (scale_of(p.a_scales, i) * scale_of(p.w_scales, j)) +
-                          (p.bias != nullptr ? Elem<Out>::get(static_cast<const Out *>(p.bias)[j]) : 0.0f)};
-            activate_all<1>(p.act, y);
-            if (p.residual != nullptr) y[0] += Elem<Out>::get(static_cast<const Out *>(p.residual)[i * p.ldr + j]);
-            static_cast<Out *>(p.out)[i * p.ldo + j] = Elem<Out>::put(y[0]);
+        };
+        float sc[V], bi[V], re[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) inputs(lo + v * LTHREADS + tid, sc[v], bi[v], re[v]);
+        g_pair_sync();
+        for (int e0 = lo + tid; e0 < hi; e0 += V * LTHREADS) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int e = e0 + v * LTHREADS;
+                if (e0 >= lo + V * LTHREADS) inputs(e, sc[v], bi[v], re[v]);
+                const long long i = i0 + e / LW, j = j0 + e % LW;
+                if (e >= hi || i >= p.m || j >= p.n) continue;
+                unsigned bits[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {  // all asked for before any is waited for
+                    bits[r] = 0u;
+                    if (r < g.split) {
+                        unsigned at;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + (unsigned)e * 4u), "r"(r));
+                        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(bits[r]) : "r"(at) : "memory");
+                    }
+                }
+                float x;
+                if constexpr (I8) {
+                    int whole = 0;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) whole += (int)bits[r];
+                    x = (float)whole;
+                } else {
+                    x = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) x += __uint_as_float(bits[r]);
+                }
+                float y[1] = {fmaf(x, sc[v], bi[v])};
+                activate_all<1>(p.act, y);
+                static_cast<Out *>(p.out)[i * p.ldo + j] = Elem<Out>::put(p.residual != nullptr ? y[0] + re[v] : y[0]);
+            }
         }
     }
     if (tid == 0 && ctl->failed != 0) {
