@@ -81,12 +81,12 @@ _stream = torch._C._cuda_getCurrentRawStream
 _F32, _I32, _I64, _I8 = (torch.float32,), (torch.int32,), (torch.int64,), (torch.int8,)
 
 
+_new = torch.empty_strided
+
+
 def _codes(x, rows, dim):
     """rows x dim int8 in rows of a multiple of 16 bytes, the padding zero: as linear reads them best."""
-    wide = (dim + 15) // 16 * 16
-    if wide == dim:
-        return x.new_empty((rows, dim), dtype=torch.int8)
-    return x.new_zeros((rows, wide), dtype=torch.int8)[:, :dim]
+    return x.new_zeros((rows, (dim + 15) // 16 * 16), dtype=torch.int8)[:, :dim]
 
 
 def rms_norm_i8(x, gain=None, *, residual=None, eps: float = 1e-6, out_codes=None, out_scales=None, out_sum=None):
@@ -103,19 +103,27 @@ def rms_norm_i8(x, gain=None, *, residual=None, eps: float = 1e-6, out_codes=Non
     if residual is not None:
         ldr = _matrix(residual, "residual", (kind,), dev, rows, dim)[2]
         r = residual.data_ptr()
-        if out_sum is None:
-            out_sum = x.new_empty((rows, dim))
+    place = x.device
     s = lds = 0
     if out_sum is not None:
         lds = _matrix(out_sum, "out_sum", (kind,), dev, rows, dim)[2]
         s = out_sum.data_ptr()
-    if out_codes is None:
-        out_codes = _codes(x, rows, dim)
+    elif residual is not None:
+        out_sum, lds = _new((rows, dim), (dim, 1), dtype=kind, device=place), dim
+        s = out_sum.data_ptr()
+    if out_codes is not None:
+        ldc = _matrix(out_codes, "out_codes", _I8, dev, rows, dim)[2]
+    elif dim % 16 == 0:
+        out_codes, ldc = _new((rows, dim), (dim, 1), dtype=torch.int8, device=place), dim
+    else:
+        out_codes, ldc = _codes(x, rows, dim), (dim + 15) // 16 * 16
     if out_scales is None:
-        out_scales = x.new_empty(rows, dtype=torch.float32)
-    ldc = _matrix(out_codes, "out_codes", _I8, dev, rows, dim)[2]
+        out_scales = _new((rows,), (1,), dtype=torch.float32, device=place)
+        scales = out_scales.data_ptr()
+    else:
+        scales = _vector(out_scales, "out_scales", _F32, dev, rows)
     st = lib.lk_rms_norm_i8(dev, _FLOATS[kind], rows, dim, x.data_ptr(), ldx, r, ldr, g, 0 if g is None else _FLOATS[gain.dtype], eps,
-                            s, lds, out_codes.data_ptr(), ldc, _vector(out_scales, "out_scales", _F32, dev, rows), _stream(dev))
+                            s, lds, out_codes.data_ptr(), ldc, scales, _stream(dev))
     if st:
         check(st)
     return out_codes, out_scales, out_sum
@@ -153,7 +161,7 @@ def linear(a, w, *, a_scales=None, w_scales=None, bias=None, act: str = "none", 
         r = residual.data_ptr()
     sa, sw, b = _vector(a_scales, "a_scales", _F32, dev, m), _vector(w_scales, "w_scales", _F32, dev, n), _vector(bias, "bias", (kind,), dev, n)
     if out is None:
-        out, ldo = a.new_empty((m, n), dtype=kind), n
+        out, ldo = _new((m, n), (n, 1), dtype=kind, device=a.device), n
     else:
         ldo = _matrix(out, "out", (kind,), dev, m, n)[2]
     st = lib.lk_linear(dev, _OPERANDS[a.dtype], m, n, k, a.data_ptr(), lda, sa, w.data_ptr(), ldw, sw, b, ACTIVATIONS[act], r, ldr,
@@ -192,8 +200,9 @@ def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, o
     mp, hold_mp = _per_row(min_p, "min_p", _F32, scores, rows, dev)
     if up is None:
         _refuse(LK_EINVAL, "u: a CUDA tensor is wanted")
-    ids = scores.new_empty(rows, dtype=torch.int64) if out_ids is None else out_ids
-    probs, kept = scores.new_empty(rows, dtype=torch.float32), scores.new_empty(rows, dtype=torch.int32)
+    place = scores.device
+    ids = _new((rows,), (1,), dtype=torch.int64, device=place) if out_ids is None else out_ids
+    probs, kept = _new((rows,), (1,), dtype=torch.float32, device=place), _new((rows,), (1,), dtype=torch.int32, device=place)
     st = lib.lk_sample(dev, _FLOATS[scores.dtype], rows, vocab, scores.data_ptr(), ld, t, k, p, mp, up,
                        _vector(ids, "out_ids", _I64, dev, rows), probs.data_ptr(), kept.data_ptr(), _stream(dev))
     if st:
