@@ -98,6 +98,9 @@ class DeviceScope {
     int prev_ = -1;
 };
 
+// rms_norm.cu: whether one of its bounded waits ran out on the current device since the last call; waits for the device.
+int norm_failed(int *out);
+
 // SMs of a device, asked once.
 inline int sm_count(int device) {
     static int known[kMaxDevices];

@@ -102,7 +102,10 @@ extern "C" int lk_linear(int device, int dtype, int64_t m, int64_t n, int64_t k,
 extern "C" int lk_ops_status(int device) {
     DeviceScope scope;
     LK_TRY(scope.enter(device, "lk_ops_status"));
-    int failed = 0;
-    LK_TRY(linear_failed(&failed));
-    return failed ? fail(LK_ETIMEOUT, "lk_linear: a bounded wait inside the kernel ran out; its results are not complete") : LK_OK;
+    int linear = 0, norm = 0;
+    LK_TRY(linear_failed(&linear));
+    LK_TRY(norm_failed(&norm));
+    if (linear) return fail(LK_ETIMEOUT, "lk_linear: a bounded wait inside the kernel ran out; its results are not complete");
+    if (norm) return fail(LK_ETIMEOUT, "lk_rms_norm_i8: a bounded wait inside the kernel ran out; its results are not complete");
+    return LK_OK;
 }
