@@ -14,11 +14,14 @@
 //
 // Two forms.  PAIR: two CTAs of a cluster share every MMA (cta_group::2, 256 rows of w), each loads its
 // own 128 rows of w and half the rows of a.  Single: one CTA per tile, and where there are too few tiles
-// to fill the GPU a cluster of `split` CTAs shares one tile's K: each sums its part, the parts are
-// exchanged through distributed shared memory, added in rank order (the result does not depend on timing),
-// and every CTA finishes its share of the columns.  No workspace, no atomics.
+// to fill the GPU a cluster of `split` CTAs shares one tile's K: each sums its part and sends every
+// other CTA its share of the columns straight from registers into shared memory (st.async, counted on the owner's
+// barrier), where the parts are added in rank order (the result does not depend on timing) and finished.  No workspace, no
+// atomics, and the cluster meets only once, while the first copies are under way.
 //
 // Every wait is bounded; a CTA that gives up raises g_linear_failed, which lk_ops_status reports.
+#include <cstddef>
+
 #include "linear.cuh"
 #include "tensor5.cuh"
 
@@ -29,7 +32,7 @@ constexpr int LSLICE = 128;         // bytes of K per stage: one swizzle row
 constexpr int LW_BYTES = LW * LSLICE;
 constexpr int LEPI_WARPS = 16;      // four per tensor-memory quadrant, 16 columns of a tile at a time each
 constexpr int LTHREADS = 64 + LEPI_WARPS * 32;
-constexpr int LMAX_STAGES = 12;
+constexpr int LMAX_STAGES = 8;        // 8,192 x 18 KB slices of an m = 8 product: 26.4 us with 8 stages, 27.6 with 6, 28.4 with 12
 constexpr int LCHUNK = 16;          // columns an epilogue thread holds at a time
 
 static __device__ unsigned g_linear_failed;  // a bounded wait ran out on this device
@@ -42,14 +45,17 @@ struct LinearTiles {
     long long tiles;
     unsigned idesc;
     unsigned columns;    // tensor memory to allocate
+    bool w_once;         // every row of w is read by one CTA only, and all of w is more than L2 would keep
 };
 
 struct LinearShared {
-    unsigned long long full[LMAX_STAGES], empty[LMAX_STAGES], acc_full[2], acc_empty[2];
-    float sa[2][256];  // the scales of a tile's rows of a, per accumulator
+    unsigned long long full[LMAX_STAGES], empty[LMAX_STAGES], acc_full[2], acc_empty[2], joined;
+    alignas(16) float sa[2][256];  // the scales of a tile's rows of a, per accumulator
     unsigned tmem_base;
     int failed;
 };
+
+static_assert(offsetof(LinearShared, sa) % 16 == 0, "read four at a time");
 
 // 2-D tiled TMA load into this CTA's shared memory, counted on `bar` (PAIR: the leader's).
 template <bool PAIR>
@@ -64,6 +70,27 @@ __device__ __forceinline__ void l_load(unsigned dst, const CUtensorMap *tm, int 
             "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
             "l"(reinterpret_cast<unsigned long long>(tm)), "r"(x), "r"(y), "r"(bar)
             : "memory");
+}
+
+// The same, the lines first to go from L2: for what is read once.
+__device__ __forceinline__ void l_load_once(unsigned dst, const CUtensorMap *tm, int x, int y, unsigned bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
+        "l"(reinterpret_cast<unsigned long long>(tm)), "r"(x), "r"(y), "r"(bar), "l"(0x12F0000000000000ull)
+        : "memory");
+}
+
+__device__ __forceinline__ unsigned l_at(unsigned local, int rank) {  // a shared-memory address as it sits in CTA `rank`
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+    return r;
+}
+// Words to another CTA's shared memory, counted on its barrier.
+__device__ __forceinline__ void l_send(unsigned to, unsigned a, unsigned b, unsigned c, unsigned d, unsigned bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void l_send(unsigned to, unsigned a, unsigned b, unsigned bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(to), "r"(a), "r"(b), "r"(bar) : "memory");
 }
 
 template <bool PAIR, bool I8>
@@ -113,7 +140,9 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
     const int a_bytes = g.mt / CG * LSLICE;
     unsigned char *sm_w = smem;                                    // [stages][128 rows][128 B]
     unsigned char *sm_a = sm_w + (size_t)g.stages * LW_BYTES;      // [stages][mt / CG rows][128 B]
-    LinearShared *ctl = reinterpret_cast<LinearShared *>(sm_a + (size_t)g.stages * a_bytes);
+    const bool joined = !PAIR && g.split > 1;
+    unsigned *sm_parts = reinterpret_cast<unsigned *>(sm_a + (size_t)g.stages * a_bytes);  // split: [CTA][columns / w][128][w] of this CTA's columns
+    LinearShared *ctl = reinterpret_cast<LinearShared *>(sm_parts + (joined ? g.mt * LW : 0));
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = PAIR || g.split > 1 ? (int)g_cta_rank() : 0;
@@ -136,12 +165,15 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
             g_mbar_init(&ctl->acc_empty[i], CG * LEPI_WARPS);
         }
         ctl->failed = 0;
+        if (joined) g_mbar_init(&ctl->joined, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (joined) g_mbar_expect_tx(&ctl->joined, (unsigned)(g.mt * LW * 4));
         if (!PAIR && first < g.tiles) {  // the first stages are on their way while the CTA sets itself up
             const int yw = (int)(first / g.tiles_m) * LW, ya = (int)(first % g.tiles_m) * g.mt;
             for (int i = 0; i < early; ++i) {
                 g_mbar_expect_tx(&ctl->full[i], (unsigned)(LW_BYTES + a_bytes));
-                l_load<PAIR>(g_smem(sm_w + (size_t)i * LW_BYTES), &tm_w, (s0 + i) * LSLICE, yw, g_smem(&ctl->full[i]));
+                if (g.w_once) l_load_once(g_smem(sm_w + (size_t)i * LW_BYTES), &tm_w, (s0 + i) * LSLICE, yw, g_smem(&ctl->full[i]));
+                else l_load<PAIR>(g_smem(sm_w + (size_t)i * LW_BYTES), &tm_w, (s0 + i) * LSLICE, yw, g_smem(&ctl->full[i]));
                 l_load<PAIR>(g_smem(sm_a + (size_t)i * a_bytes), &tm_a, (s0 + i) * LSLICE, ya, g_smem(&ctl->full[i]));
             }
         }
@@ -159,6 +191,7 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (PAIR) g_pair_sync();  // the partner's barriers exist before anything is signalled across
+    if (joined) asm volatile("barrier.cluster.arrive;" ::: "memory");  // so do the others'; waited for before the first word is sent
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = ctl->tmem_base;
     volatile int *failed = &ctl->failed;
@@ -172,12 +205,19 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
             const int yw = (int)(t / g.tiles_m) * LW * CG + cta_of * LW;
             const int ya = (int)(t % g.tiles_m) * g.mt + cta_of * (g.mt / CG);
             for (int s = s0; s < s1; ++s) {
+                if (t == first && s - s0 < early) {
+                    // already asked for.  Its stage must not be waited for either: it may have been used and freed by
+                    // now, and the wait would be for the phase after that
+                    if (++stage == g.stages) stage = 0, phase ^= 1u;
+                    continue;
+                }
                 ok = g_mbar_wait_warp(&ctl->empty[stage], phase ^ 1u, failed);
                 if (!ok) break;
-                if (!(t == first && s - s0 < early) && g_elect_one()) {
+                if (g_elect_one()) {
                     const unsigned bar = PAIR ? g_leader_addr(g_smem(&ctl->full[stage])) : g_smem(&ctl->full[stage]);
                     if (cta_of == 0) g_mbar_expect_tx(&ctl->full[stage], (unsigned)(CG * (LW_BYTES + a_bytes)));
-                    l_load<PAIR>(g_smem(sm_w + (size_t)stage * LW_BYTES), &tm_w, s * LSLICE, yw, bar);
+                    if (!PAIR && g.w_once) l_load_once(g_smem(sm_w + (size_t)stage * LW_BYTES), &tm_w, s * LSLICE, yw, bar);
+                    else l_load<PAIR>(g_smem(sm_w + (size_t)stage * LW_BYTES), &tm_w, s * LSLICE, yw, bar);
                     l_load<PAIR>(g_smem(sm_a + (size_t)stage * a_bytes), &tm_a, s * LSLICE, ya, bar);
                 }
                 __syncwarp();
@@ -221,7 +261,6 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
         const int et = tid - 64;
         const long long ldr = p.ldr * (long long)sizeof(Out), ldo = p.ldo * (long long)sizeof(Out);
         bool epi_ok = true;
-        const bool joined = !PAIR && g.split > 1;
         int acc = 0;
         unsigned acc_phase = 0;
         for (long long t = first; t < g.tiles; t += step) {
@@ -250,11 +289,13 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
             }
             if (!g_mbar_wait_warp(&ctl->acc_full[acc], acc_phase, failed)) epi_ok = false;
             if (!epi_ok) {
+                if (joined) asm volatile("barrier.cluster.wait;" ::: "memory");
                 // the other warps of the epilogue may be waiting at the barrier above: stay with them to the last tile
                 if (++acc == 2) acc = 0, acc_phase ^= 1u;
                 continue;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (joined) asm volatile("barrier.cluster.wait;" ::: "memory");
             for (int c = part * LCHUNK; c < g.mt; c += 4 * LCHUNK) {
                 unsigned v[LCHUNK];
                 l_tmem_ld16(tmem + (unsigned)(acc * g.mt + c) + ((unsigned)(quad * 32) << 16), v);
@@ -265,10 +306,21 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
                     if (c + 4 * LCHUNK < g.mt) fetch(c + 4 * LCHUNK);
                 }
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (joined) {  // this CTA's part of the sums, to where the cluster can read it
-                    unsigned *red = reinterpret_cast<unsigned *>(smem) + c * LW + quad * 32 + lane;
+                if (joined) {  // this CTA's part of the sums, to the CTAs whose columns these are
+                    const int own = g.mt / g.split, n = quad * 32 + lane;
+                    if (own >= 4) {
 #pragma unroll
-                    for (int u = 0; u < LCHUNK; ++u) red[u * LW] = v[u];
+                        for (int u = 0; u < LCHUNK; u += 4) {
+                            const int to = (c + u) / own, at = ((part_of * own + (c + u) % own) >> 2) * LW + n;
+                            l_send(l_at(g_smem(sm_parts + 4 * at), to), v[u], v[u + 1], v[u + 2], v[u + 3], l_at(g_smem(&ctl->joined), to));
+                        }
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < LCHUNK; u += 2) {
+                            const int to = (c + u) / own, at = ((part_of * own + (c + u) % own) >> 1) * LW + n;
+                            l_send(l_at(g_smem(sm_parts + 2 * at), to), v[u], v[u + 1], l_at(g_smem(&ctl->joined), to));
+                        }
+                    }
                     continue;
                 }
                 if (p.a_scales != nullptr) {
@@ -309,69 +361,64 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
         }
     }
     // ------------------------------ joining the parts of K ------------------------------
+    if (joined && warp >= 2) {  // one tile per cluster; this CTA's columns are mt / split of it
+        const int own = g.mt / g.split, w = own >= 4 ? 4 : 2, items = own / w * LW;
+        const long long j0 = (first / g.tiles_m) * LW, i0 = (first % g.tiles_m) * g.mt + part_of * own;
+        bool ok = true, waited = false;
+        for (int e = tid - 64; e < items; e += LEPI_WARPS * 32) {  // one column of the result, w rows of it
+            const int n = e % LW;
+            const long long i = i0 + e / LW * w, j = j0 + n;
+            const bool live = j < p.n;
+            // the epilogue's inputs are on their way while the parts are
+            const float sw = live ? scale_of(p.w_scales, j) : 0.0f;
+            const float bias = live && p.bias != nullptr ? Elem<Out>::get(static_cast<const Out *>(p.bias)[j]) : 0.0f;
+            float sa[4], r[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool there = live && u < w && i + u < p.m;
+                sa[u] = there ? scale_of(p.a_scales, i + u) : 0.0f;
+                r[u] = there && p.residual != nullptr ? Elem<Out>::get(static_cast<const Out *>(p.residual)[(i + u) * p.ldr + j]) : 0.0f;
+            }
+            if (!waited) ok = g_mbar_wait(&ctl->joined, 0u, failed), waited = true;
+            if (!ok) break;
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            int whole[4] = {0, 0, 0, 0};
+            for (int q = 0; q < g.split; ++q) {
+                unsigned v[4] = {0u, 0u, 0u, 0u};
+                if (w == 4) {
+                    const uint4 f = *reinterpret_cast<const uint4 *>(sm_parts + 4 * ((q * own >> 2) * LW + e));
+                    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+                } else {
+                    const uint2 f = *reinterpret_cast<const uint2 *>(sm_parts + 2 * ((q * own >> 1) * LW + e));
+                    v[0] = f.x, v[1] = f.y;
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if constexpr (I8) whole[u] += (int)v[u];
+                    else x[u] += __uint_as_float(v[u]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = fmaf(I8 ? (float)whole[u] : x[u], sa[u] * sw, bias);
+            activate_all<4>(p.act, x);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (live && u < w && i + u < p.m)
+                    static_cast<Out *>(p.out)[(i + u) * p.ldo + j] = Elem<Out>::put(p.residual != nullptr ? x[u] + r[u] : x[u]);
+        }
+        // whoever had nothing to finish waits too: this CTA's shared memory is written to until all parts are here
+        if (!waited) g_mbar_wait(&ctl->joined, 0u, failed);
+    }
+    if (joined && warp < 2) asm volatile("barrier.cluster.wait;" ::: "memory");
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (!PAIR && g.split > 1) {  // one tile per cluster
-        const long long j0 = (first / g.tiles_m) * LW, i0 = (first % g.tiles_m) * g.mt;
-        const int lo = g.mt * part_of / g.split * LW, hi = g.mt * (part_of + 1) / g.split * LW;
-        const unsigned base = g_smem(smem);
-        // what the epilogue needs is on its way while the cluster meets; LTHREADS is a multiple of neither, so each value
-        // has a thread of its own
-        constexpr int V = 4;
-        const auto inputs = [&](int e, float &s, float &b, float &r) {
-            const long long i = i0 + e / LW, j = j0 + e % LW;
-            s = 1.0f, b = r = 0.0f;
-            if (e < hi && i < p.m && j < p.n) {
-                s = scale_of(p.a_scales, i) * scale_of(p.w_scales, j);
-                if (p.bias != nullptr) b = Elem<Out>::get(static_cast<const Out *>(p.bias)[j]);
-                if (p.residual != nullptr) r = Elem<Out>::get(static_cast<const Out *>(p.residual)[i * p.ldr + j]);
-            }
-        };
-        float sc[V], bi[V], re[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) inputs(lo + v * LTHREADS + tid, sc[v], bi[v], re[v]);
-        g_pair_sync();
-        for (int e0 = lo + tid; e0 < hi; e0 += V * LTHREADS) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int e = e0 + v * LTHREADS;
-                if (e0 >= lo + V * LTHREADS) inputs(e, sc[v], bi[v], re[v]);
-                const long long i = i0 + e / LW, j = j0 + e % LW;
-                if (e >= hi || i >= p.m || j >= p.n) continue;
-                unsigned bits[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {  // all asked for before any is waited for
-                    bits[r] = 0u;
-                    if (r < g.split) {
-                        unsigned at;
-                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + (unsigned)e * 4u), "r"(r));
-                        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(bits[r]) : "r"(at) : "memory");
-                    }
-                }
-                float x;
-                if constexpr (I8) {
-                    int whole = 0;
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) whole += (int)bits[r];
-                    x = (float)whole;
-                } else {
-                    x = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) x += __uint_as_float(bits[r]);
-                }
-                float y[1] = {fmaf(x, sc[v], bi[v])};
-                activate_all<1>(p.act, y);
-                static_cast<Out *>(p.out)[i * p.ldo + j] = Elem<Out>::put(p.residual != nullptr ? y[0] + re[v] : y[0]);
-            }
-        }
-    }
     if (tid == 0 && ctl->failed != 0) {
         atomicExch(&g_linear_failed, 1u);
         // copies this CTA issued may still be landing in its shared memory: give them time before it is released
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000ll) {}
     }
-    if (PAIR || g.split > 1) g_pair_sync();  // nothing of the cluster is still aimed at, or reading, this CTA
+    if (PAIR) g_pair_sync();  // nothing of the partner is still aimed at this CTA's barriers or tensor memory
     if (warp == 1) {
         __syncwarp();
         if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.columns) : "memory");
@@ -455,7 +502,7 @@ template <bool PAIR, bool I8, typename Out>
 static int mma_launch(const CUtensorMap &tw, const CUtensorMap &ta, const LinearArgs &p, const LinearTiles &g, int device, int sms, cudaStream_t st) {
     constexpr int CG = PAIR ? 2 : 1;
     static bool sized[kMaxDevices];
-    const size_t smem = (size_t)g.stages * (LW_BYTES + g.mt / CG * LSLICE) + sizeof(LinearShared) + 1024;
+    const size_t smem = (size_t)g.stages * (LW_BYTES + g.mt / CG * LSLICE) + (g.split > 1 ? g.mt * LW * 4 : 0) + sizeof(LinearShared) + 1024;
     if (!sized[device]) {
         LK_CUDA(cudaFuncSetAttribute((const void *)k_linear_mma<PAIR, I8, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
         sized[device] = true;
@@ -495,7 +542,9 @@ int linear_mma_launch(const LinearArgs &p, int dtype, int device, cudaStream_t s
     g.tiles_m = (int)((p.m + g.mt - 1) / g.mt);
     g.tiles = g.tiles_m * ((p.n + LW * cg - 1) / (LW * cg));
     const int stage_bytes = LW_BYTES + g.mt / cg * LSLICE;
-    g.stages = std::min((226 * 1024 - (int)sizeof(LinearShared) - 1024) / stage_bytes, LMAX_STAGES);
+    g.stages = std::min((226 * 1024 - (int)sizeof(LinearShared) - 1024 - (g.split > 1 ? g.mt * LW * 4 : 0)) / stage_bytes, LMAX_STAGES);
+    // 134 MB of w: 25.1 us with the hint, 26.4 without; 17 MB, which the next call may find in L2: 9.1 us with, 7.3 without
+    g.w_once = g.tiles_m == 1 && p.n * p.k * eb > (64ll << 20);
     g.columns = std::max(32u, 2u * (unsigned)g.mt);
     const unsigned kinds = dtype == LK_I8 ? (2u << 4) | (1u << 7) | (1u << 10)  // int8 x int8 -> int32
                            : dtype == LK_BF16 ? (1u << 4) | (1u << 7) | (1u << 10) : (1u << 4);  // -> float32

@@ -255,3 +255,20 @@ def test_refusals(ops, lk):
         p.update(kw)
         with pytest.raises(lk.LokiError):
             ops.linear(p.pop("a"), p.pop("w"), **p)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.bfloat16])
+def test_few_slices_many_times(ops, dtype):
+    """Products whose copies are all asked for at once: a stage may be used and freed before the warp that asks looks at it."""
+    for m, n, k in [(17, 1000, 771), (1, 1000, 300), (40, 512, 1030), (64, 300, 200), (130, 700, 130)]:
+        g, a, w, sa, sw = operands(m, n, k, dtype, k)
+        first = verify(ops, a, w, torch.float32, sa, sw)
+        for _ in range(100):
+            again = ops.linear(a, w, a_scales=sa, w_scales=sw, out_dtype=torch.float32)
+        assert torch.equal(first, again)
+        ops.check_device()
+
+
+def test_no_wait_has_run_out(ops):
+    """All calls of this file: none gave up waiting for a copy."""
+    ops.check_device()
