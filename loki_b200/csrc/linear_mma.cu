@@ -191,7 +191,9 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (PAIR) g_pair_sync();  // the partner's barriers exist before anything is signalled across
-    if (joined) asm volatile("barrier.cluster.arrive;" ::: "memory");  // so do the others'; waited for before the first word is sent
+    // so do the others'; waited for before the first word is sent.  Relaxed: the fence behind the barriers' set-up is all that
+    // has to be seen, and a release by every thread held up the first MMAs
+    if (joined) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = ctl->tmem_base;
     volatile int *failed = &ctl->failed;
@@ -471,11 +473,16 @@ static int cluster_room(int device, const ClusterRoom **out) {
     return 0;
 }
 
+// Stages of a ring beside the parts of K that arrive from the cluster.
+static int ring_stages(int mt, int cg, int split) {
+    return std::min((226 * 1024 - (int)sizeof(LinearShared) - 1024 - (split > 1 ? mt * LW * 4 : 0)) / (LW_BYTES + mt / cg * LSLICE), LMAX_STAGES);
+}
+
 // The tile that finishes first, by an account of one CTA's clocks whose constants were fitted to 110 shapes (m 1 to 1,024,
-// five n x k, int8 and bf16) with every tile timed; over them the choice costs 0.3 % against the best tile, 8 % at worst.
-// A slice of K: its MMAs, its bytes at 57 per clock and SM (of all CTAs together 5,770 per clock), never under 515 clocks.
-// A tile's epilogue, 31 clocks per row of a, runs under the next tile's slices; the last one shows.  An exchange of
-// parts costs 3,750 clocks and 35 per row of a.
+// five n x k, int8 and bf16) with every tile timed; over them the choice costs 0.2 % against the best tile, 4 % at worst.
+// A slice of K: its MMAs (0.62 clocks per row of a), its bytes at 58 per clock and SM and 5,456 for all CTAs together, and the
+// 4,058 clocks from asking for a slice to having it, shared by the stages.  A tile's epilogue, 31 clocks per row of a, runs under
+// the next tile's slices; the last one shows.  Joining parts of K costs 4,305 clocks and 16 per row of a.
 static LinearPlan linear_plan(long long m, long long n, int slices, const ClusterRoom &room) {
     LinearPlan best = {false, 16, 1};
     double least = 1e300;
@@ -483,11 +490,13 @@ static LinearPlan linear_plan(long long m, long long n, int slices, const Cluste
         const int cg = pair ? 2 : 1, per = cg * split;
         const long long tiles = ((m + mt - 1) / mt) * ((n + LW * cg - 1) / (LW * cg));
         if (room.of[per] < 1 || (split > 1 && (tiles > room.of[per] || split > slices))) return;
+        const int stages = ring_stages(mt, cg, split);
+        if (stages < 1) return;
         const double waves = (double)((tiles + room.of[per] - 1) / room.of[per]);
         const double bytes = LW_BYTES + mt / cg * LSLICE, active = (double)std::min<long long>(tiles * per, room.of[1]);
-        const double slice = std::max(std::max(0.68 * mt, 515.0), std::max(bytes / 57.0, active * bytes / 5770.0));
+        const double slice = std::max(std::max(0.62 * mt, 4058.0 / stages), std::max(bytes / 58.0, active * bytes / 5456.0));
         const double main = (slices + split - 1) / split * slice, epilogue = 31.0 * mt / split;
-        const double cost = waves * (waves > 1.0 ? std::max(main, epilogue) : main) + epilogue + (split > 1 ? 3750.0 + 35.0 * mt : 0.0);
+        const double cost = waves * (waves > 1.0 ? std::max(main, epilogue) : main) + epilogue + (split > 1 ? 4305.0 + 16.0 * mt : 0.0);
         if (cost < least) least = cost, best = {pair, mt, split};
     };
     for (int mt = 16; mt <= 256; mt *= 2) {
@@ -541,9 +550,8 @@ int linear_mma_launch(const LinearArgs &p, int dtype, int device, cudaStream_t s
     g.split = plan.split;
     g.tiles_m = (int)((p.m + g.mt - 1) / g.mt);
     g.tiles = g.tiles_m * ((p.n + LW * cg - 1) / (LW * cg));
-    const int stage_bytes = LW_BYTES + g.mt / cg * LSLICE;
-    g.stages = std::min((226 * 1024 - (int)sizeof(LinearShared) - 1024 - (g.split > 1 ? g.mt * LW * 4 : 0)) / stage_bytes, LMAX_STAGES);
-    // 134 MB of w: 25.1 us with the hint, 26.4 without; 17 MB, which the next call may find in L2: 9.1 us with, 7.3 without
+    g.stages = ring_stages(g.mt, cg, g.split);
+    // 134 MB of w: 25.1 us with the hint, 26.4 without; 17 MB: no difference, and the next call may find it in L2
     g.w_once = g.tiles_m == 1 && p.n * p.k * eb > (64ll << 20);
     g.columns = std::max(32u, 2u * (unsigned)g.mt);
     const unsigned kinds = dtype == LK_I8 ? (2u << 4) | (1u << 7) | (1u << 10)  // int8 x int8 -> int32
