@@ -157,12 +157,14 @@ struct Row {
     float bottom;   // a score so far below it that it weighs nothing
     bool alone;     // nothing else weighs: it is +infinity, or T is that small
     double top_wide;
-    double octaves; // 64 / (T ln 2): a distance in 64ths of an octave
+    double octaves; // 64 / (T ln 2): a score in 64ths of an octave
+    double whole;   // 1.5 * 2^52 - N: adding it rounds to a whole number in the low word
+    unsigned scale_bits;  // exponent of 2^F
     float temp, per_t;  // T, 1 / T
     u64 floor;      // min_p: the lowest key that it keeps
     u64 thr;        // entries with a key at or above this are kept
     float thr_x;    // its score and its index
-    unsigned thr_i;
+    int thr_i;
 
     __device__ __forceinline__ void sync() const {
         if (a.ctas > 1) {
@@ -175,31 +177,34 @@ struct Row {
     __device__ __forceinline__ void keep_from(u64 k) {
         thr = k;
         thr_x = f32_from_ord(key_ord(k));
-        thr_i = key_slot(k);
+        thr_i = (int)min((long long)key_slot(k) - start, 0x7fffffffll);  // as a local index
     }
     // NaN compares false; -infinity is below every threshold
-    __device__ __forceinline__ bool kept(float v, int i) const { return v > thr_x || (v == thr_x && (unsigned)(start + i) <= thr_i); }
+    __device__ __forceinline__ bool kept(float v, int i) const { return v > thr_x || (v == thr_x && i <= thr_i); }
     __device__ __forceinline__ float entry(int i) const { return Elem<T>::get(i < a.cap ? data[i] : x[i]); }
 
-    // w * 2^F of a score, rounded, where others than the largest weigh.  Tang's scheme (ACM TOMS 15, 1989): with y =
-    // (x - max) / T / ln 2 * 64 = n + r, n whole, |r| <= 1/2:  w = 2^(n div 64) * 2^((n mod 64) / 64) * e^(r ln 2 / 64), the
-    // middle factor from a table, the last by its series to the fourth power (next term 4e-14).  The roundings to whole
-    // numbers are done by adding constants, the power of two on the bits: conversions issue at an eighth of the rate.
-    __device__ __forceinline__ u64 weight(float v) const {
-        const double whole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number in the low word
-        const double dx = (double)fmaxf(v, bottom) - top_wide;
-        const double t = fma(dx, octaves, whole);
-        const double r = fma(dx, octaves, -(t - whole));
+    // w * 2^F of a score, rounded, where others than the largest weigh.  Tang's scheme (ACM TOMS 15, 1989): with y = x / T / ln 2 *
+    // 64 = N + n + r, n whole, |r| <= 1/2, N the whole number next to the largest y:  w = 2^(n div 64) * 2^((n mod 64) / 64) *
+    // e^(r ln 2 / 64), the middle factor from a table, the last by its series to the fourth power (next term 4e-14).  All weights
+    // of a row share a factor within 2^(1/128) of 1 (the largest y is not whole), which no quotient of weights sees.  Roundings to
+    // whole numbers are done by adding constants, the power of two on the bits: conversions issue at an eighth of the rate.
+    // The result still carries the exponent bits of the last addition: kTag more than the weight.
+    static constexpr u64 kTag = 0x4330000000000000ull;  // 2^52 as a float64
+    __device__ __forceinline__ u64 tagged(float v) const {
+        const double x = (double)fmaxf(v, bottom);
+        const double t = fma(x, octaves, whole);
+        const double r = fma(x, octaves, whole - t);
         const int n = __double2loint(t);
         constexpr double c = 0.693147180559945309417232 / 64;
         double q = fma(r, c * c * c * c / 24, c * c * c / 6);
         q = fma(r, q, c * c / 2);
         q = fma(r, q, c);
         q = fma(r, q, 1.0);
-        const double scale = __hiloint2double(((n & ~63) << 14) + ((1023 + a.unit_bits) << 20), 0);
-        const double w = fma(s.octave[n & 63] * q, scale, 4503599627370496.0);  // + 2^52; w <= 2^50
-        return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+        const double scale = __hiloint2double((int)(((unsigned)n * (1u << 14) + scale_bits) & 0xfff00000u), 0);
+        return (u64)__double_as_longlong(fma(s.octave[n & 63] * q, scale, 4503599627370496.0));  // + 2^52; w < 2^51
     }
+    __device__ __forceinline__ u64 weight(float v) const { return tagged(v) - kTag; }
+    // The same for any row.
     __device__ __forceinline__ u64 weight_of(float v) const {
         if (alone) return v == top ? 1ull << a.unit_bits : 0ull;
         return weight(v);
@@ -245,19 +250,33 @@ struct Row {
     }
 
     // Sum over the entries with keep(score, index) of their weights (MASS) or their number; warp_w keeps this CTA's warps'
-    // sums and slot_w the CTAs'.
+    // sums and slot_w the CTAs'.  *mine: how many of this thread's entries there are.
     template <bool MASS, typename K>
-    __device__ __forceinline__ u64 sums(K keep) const {
+    __device__ __forceinline__ u64 sums(K keep, unsigned *mine) const {
         u64 w = 0;
+        unsigned n = 0;
         each([&](const float (&v)[4], int i) {
             bool k[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) k[e] = keep(v[e], i + e);
             if (!(k[0] | k[1] | k[2] | k[3])) return;
-            u64 m[4] = {k[0], k[1], k[2], k[3]};
-            if (MASS) weights(v, k, m);
-            w += (m[0] + m[1]) + (m[2] + m[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) n += k[e];
+            if (!MASS) return;
+            if (alone) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w += k[e] && v[e] == top ? 1ull << a.unit_bits : 0ull;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const u64 m = tagged(v[e]);
+                    w += k[e] ? m : 0ull;
+                }
+            }
         });
+        *mine = n;
+        if (!MASS) w = n;
+        else if (!alone) w -= n * kTag;
         w = warp_sum(w);
         __syncthreads();
         if (lane == 0) s.warp_w[warp] = w;
@@ -583,7 +602,8 @@ struct Row {
                 const u64 need = (want - base + each_w - 1) / each_w;  // each_w > 0: the bin reaches the target
                 if (need < n) {
                     const auto tie = [&](float v, int i) { return v == tied && kept(v, i); };
-                    sums<false>(tie);
+                    unsigned none;
+                    sums<false>(tie, &none);
                     walk<false>(tie, need - 1);
                     if (tid == 0 && s.found >= 0)
                         for (int r = 0; r < a.ctas; ++r) s_put(s_at(&s.cut, r), key(tied, s.found));
@@ -676,6 +696,8 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     w.top_wide = (double)w.top;
     w.temp = temp;
     w.octaves = 64.0 / (0.693147180559945309417232 * (double)temp);
+    w.whole = 6755399441055744.0 - rint(w.top_wide * w.octaves);
+    w.scale_bits = (unsigned)(1023 + a.unit_bits) << 20;
     w.per_t = fminf(1.0f / temp, 3e38f);
     // 62 octaves down a weight rounds to 0 (F <= 50).  Where the next lower float32 is further down than that, nothing but the
     // largest score weighs; else `bottom` is 62 to 124 octaves down, or the lowest score there is.
@@ -710,13 +732,9 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
 
     // ---- the draw ----
     unsigned count = 0;
-    const auto keep = [&](float v, int i) {
-        const bool yes = w.kept(v, i);
-        count += yes;
-        return yes;
-    };
+    const auto keep = [&](float v, int i) { return w.kept(v, i); };
     w.keep_from(max(w.thr, w.floor));
-    all = w.template sums<true>(keep);
+    all = w.template sums<true>(keep, &count);
     count = __reduce_add_sync(0xffffffffu, count);
     if (lane == 0) s.warp_n[warp] = count;
     w.template walk<true>(keep, Row<T>::aim(u, all));
