@@ -64,7 +64,7 @@ struct alignas(16) SampleShared {
     unsigned slot_top[SMAX_CTAS], slot_n[SMAX_CTAS], slot_a[SMAX_CTAS], slot_b[SMAX_CTAS];
     unsigned noted;
     u64 cut;                                   // a decision of the first CTA, or of the one that holds an entry
-    u64 found_w, found_before;
+    u64 found_w, found_before, floor;
     int found;
 };
 
@@ -305,10 +305,9 @@ struct Row {
         if (!mine) return;
         int lo = 0, n = wlen;  // first the stretch of a warp, then a 32nd of that, then its entries
         for (int level = 0;; ++level) {
-            int at = 0;
-            u64 run = before;
-            for (; at < SWARPS - 1 && run + s.warp_w[at] <= target; ++at) run += s.warp_w[at];
-            before = run;
+            const u64 w_at = s.warp_w[lane], inc_at = warp_scan(w_at, lane) + before;
+            const int at = __ffs(__ballot_sync(0xffffffffu, inc_at > target)) - 1;
+            before = shfl_u64(inc_at - w_at, at);
             lo += at * n;
             if (level == 1) break;
             const int end = min(lo + n, len);
@@ -370,17 +369,22 @@ struct Row {
             if (a.kept) a.kept[row] = count;
         }
     }
-    // The lowest key with w >= min_p, i.e. (x - max) / T >= log(min_p): by bisection over the images.
+    // The lowest key with w >= min_p, i.e. (x - max) / T >= log(min_p): a warp tries 32 images at a time.
     __device__ __forceinline__ u64 lowest(float min_p) const {
-        if (min_p <= 0.0f) return 0ull;
         const double end = log((double)min_p);
         unsigned lo = kNegInf + 1, hi = ord_from_f32(top);  // the largest score is always kept
         while (lo < hi) {
-            const unsigned mid = lo + (hi - lo) / 2;
-            if (((double)f32_from_ord(mid) - top_wide) * (octaves * (0.693147180559945309417232 / 64)) >= end) hi = mid;
-            else lo = mid + 1;
+            const unsigned step = (hi - lo) / 32 + 1, mid = lo + min(lane * step, hi - lo);
+            const bool in = mid == hi || ((double)f32_from_ord(mid) - top_wide) * (octaves * (0.693147180559945309417232 / 64)) >= end;
+            const int first = __ffs(__ballot_sync(0xffffffffu, in)) - 1;  // lanes ascend: the first that is kept, if any
+            if (first < 0) lo += 31 * step + 1;
+            else {
+                hi = __shfl_sync(0xffffffffu, mid, first);
+                if (first > 0) lo = __shfl_sync(0xffffffffu, mid, first - 1) + 1;
+                else break;  // lo itself
+            }
         }
-        return make_key(lo, ~0u);
+        return make_key(hi, ~0u);
     }
     static __device__ __forceinline__ u64 aim(float u, u64 total) {
         const double t = (double)u * (double)total;
@@ -645,6 +649,11 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     if (tid < 64) s.octave[tid] = exp2(tid / 64.0);
     if (a.ctas > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");  // waited for before the first write to another CTA
 
+    w.temp = temp;
+    w.octaves = 64.0 / (0.693147180559945309417232 * (double)temp);
+    w.per_t = fminf(1.0f / temp, 3e38f);
+    w.scale_bits = (unsigned)(1023 + a.unit_bits) << 20;
+
     // ---- the row comes in; its largest score ----
     const int held = min(w.len, a.cap);
     unsigned own = 0;  // the largest that this thread has seen
@@ -694,17 +703,21 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     }
     w.top = f32_from_ord(top);
     w.top_wide = (double)w.top;
-    w.temp = temp;
-    w.octaves = 64.0 / (0.693147180559945309417232 * (double)temp);
     w.whole = 6755399441055744.0 - rint(w.top_wide * w.octaves);
-    w.scale_bits = (unsigned)(1023 + a.unit_bits) << 20;
-    w.per_t = fminf(1.0f / temp, 3e38f);
     // 62 octaves down a weight rounds to 0 (F <= 50).  Where the next lower float32 is further down than that, nothing but the
     // largest score weighs; else `bottom` is 62 to 124 octaves down, or the lowest score there is.
     const double deep = 62.0 * 0.693147180559945309417232 * (double)temp;
     w.alone = !(w.top_wide - (double)nextafterf(w.top, -CUDART_INF_F) < deep);  // true for +infinity
     w.bottom = __double2float_rd(fmax(w.top_wide - deep, -(double)FLT_MAX));
-    w.floor = w.lowest(least_in);
+    w.floor = 0ull;
+    if (least_in > 0.0f) {
+        if (warp == 0) {
+            const u64 f = w.lowest(least_in);
+            if (lane == 0) s.floor = f;
+        }
+        __syncthreads();
+        w.floor = s.floor;
+    }
     w.keep_from(make_key(kNegInf + 1, 0xffffffffu - 1u));
 
     // ---- few candidates ----
