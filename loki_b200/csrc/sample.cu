@@ -60,7 +60,9 @@ struct alignas(16) SampleShared {
     double octave[64];                         // 2^(j/64)
     u64 warp_w[SWARPS];
     unsigned warp_n[SWARPS];
-    u64 slot_w[SMAX_CTAS];                     // one word from every CTA of the row
+    u64 above_w[SWARPS];                       // look(): what lies above the cut's place, by warp
+    unsigned above_n[SWARPS];
+    u64 slot_w[SMAX_CTAS], slot_v[SMAX_CTAS];  // one word from every CTA of the row
     unsigned slot_top[SMAX_CTAS], slot_n[SMAX_CTAS], slot_a[SMAX_CTAS], slot_b[SMAX_CTAS];
     unsigned noted;
     u64 cut;                                   // a decision of the first CTA, or of the one that holds an entry
@@ -161,6 +163,7 @@ struct Row {
     double whole;   // 1.5 * 2^52 - N: adding it rounds to a whole number in the low word
     unsigned scale_bits;  // exponent of 2^F
     float temp, per_t;  // T, 1 / T
+    unsigned split;     // 0, or the distance (its bits) above which look() has summed the weights by warp
     u64 floor;      // min_p: the lowest key that it keeps
     u64 thr;        // entries with a key at or above this are kept
     float thr_x;    // its score and its index
@@ -277,6 +280,7 @@ struct Row {
         *mine = n;
         if (!MASS) w = n;
         else if (!alone) w -= n * kTag;
+        if (MASS && split != 0 && lane == 0) w += s.above_w[warp], *mine += s.above_n[warp];
         w = warp_sum(w);
         __syncthreads();
         if (lane == 0) s.warp_w[warp] = w;
@@ -489,6 +493,89 @@ struct Row {
         return 0ull;
     }
 
+    // The first look of a cut by weight, at the price of one pass over the weights: the entries of each bin are counted, which
+    // with the mean weight of a bin says to a thousandth where the cut is, and then one pass sums the kept weights of all, of what
+    // lies above the three bins around that place (by warp, for the draw), and bins those three finely.  The sums are exact:
+    // they show whether the cut is in there (1: found_before and all_n, all_w of the fine bins from `start` on are set), else the
+    // cut is made from the beginning (0).  2: there are at most SLIST entries down to there, and they are in the lists.
+    __device__ __forceinline__ int look(float p, bool whole_row, u64 *all, u64 *want, unsigned *start, int *listed) {
+        clear_bins<false>();
+        each([&](const float (&v)[4], int i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (kept(v[e], i + e)) atomicAdd(&s.n[first_bin(distance(v[e]))], 1u);
+        });
+        join_bins<false>();
+        const auto edge = [](int b) { return __uint_as_float((unsigned)(SD_BASE + b) << SD_SHIFT); };
+        const float lo = tid == 0 ? 0.0f : edge(tid), hi = edge(tid + 1);
+        const float mean = (__expf(-lo) - __expf(-hi)) / (hi - lo);
+        const u64 m = __float2ull_rn((float)s.all_n[tid] * mean * 1073741824.0f);
+        const u64 inc = block_scan(s, m);
+        if (tid == ST - 1) s.cut = inc;
+        __syncthreads();
+        const int b = reach(m, 0ull, max((u64)((double)fmaxf(p, 0.0f) * (double)s.cut), (u64)1));
+        if (b < 0 || b >= SBINS - 2) return 0;
+        const u64 upto = block_scan(s, tid <= b + 1 ? s.all_n[tid] : 0u);
+        if (tid == ST - 1) s.found_w = upto;
+        __syncthreads();
+        const bool few = whole_row && s.found_w <= SLIST;
+        if (!few && b < 2) return 0;  // the first bin is not one of distances alike
+        const unsigned first = few ? 0u : (unsigned)(SD_BASE + b - 1) << SD_SHIFT, end = (unsigned)(SD_BASE + b + 2) << SD_SHIFT;
+        __syncthreads();
+        clear_bins<true>();
+        u64 w_all = 0, w_above = 0;
+        unsigned n_above = 0;
+        each([&](const float (&v)[4], int i) {
+            bool k[4], in[4];
+            u64 w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = kept(v[e], i + e);
+            if (!(k[0] | k[1] | k[2] | k[3])) return;
+            weights(v, k, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned d = distance(v[e]);
+                const bool above = k[e] && d < (few ? end : first);
+                in[e] = k[e] && d < end && d >= first;
+                w_all += w[e];
+                w_above += above ? w[e] : 0ull;
+                n_above += above;
+                if (in[e] && !few) {
+                    const int at = (int)((d - first) >> (SD_SHIFT - 8));
+                    atomicAdd(&s.n[at], 1u);
+                    const unsigned l = (unsigned)w[e], old = atomicAdd(&s.lo[at], l);
+                    const unsigned h = (unsigned)(w[e] >> 32) + (old + l < l ? 1u : 0u);
+                    if (h) atomicAdd(&s.hi[at], h);
+                }
+            }
+            if (few) note(in, v, i);
+        });
+        w_all = warp_sum(w_all);
+        w_above = warp_sum(w_above);
+        n_above = __reduce_add_sync(0xffffffffu, n_above);
+        if (lane == 0) s.warp_w[warp] = w_all, s.above_w[warp] = w_above, s.above_n[warp] = n_above;
+        __syncthreads();
+        if (warp == 0) {
+            w_all = warp_sum(s.warp_w[lane]);
+            w_above = warp_sum(s.above_w[lane]);
+            if (lane < a.ctas) {
+                s_put(s_at(&s.slot_w[rank], lane), w_all);
+                s_put(s_at(&s.slot_v[rank], lane), w_above);
+            }
+        }
+        if (few) *listed = (int)deliver();
+        else join_bins<true>();
+        u64 above = 0;
+        *all = 0;
+        for (int r = 0; r < a.ctas; ++r) *all += s.slot_w[r], above += s.slot_v[r];
+        *want = p <= 0.0f ? 1ull : max((u64)ceil((double)p * (double)*all), (u64)1);
+        sync();  // the slots may be written again
+        if (few) return above >= *want ? 2 : 0;
+        if (above >= *want || reach(s.all_w[tid], above, *want) < 0) return 0;
+        *start = first;
+        return 1;
+    }
+
     // MASS: moves thr up to the last entry of the shortest prefix that holds the share p of the kept weight.
     // Else: to the k-th entry.  Returns the number of candidates when all that may be kept is in the
     // lists instead (`whole`: thr is still at the row's end), with the row's weight in *all; 0 when thr has been moved.
@@ -498,18 +585,27 @@ struct Row {
         // the entries looked at: d >> in == pre (by distance), or image in [olo, ohi]; their bins: (d >> sub) - from
         int in = 31, sub = SD_SHIFT;
         unsigned pre = 0, from = SD_BASE, olo = 0, ohi = 0;
-        bool by_image = false;
-        for (int level = 0;; ++level) {
-            clear_bins<MASS>();
+        bool by_image = false, looked = false;
+        if (MASS && !alone) {
+            int listed;
+            const int seen = look(p, whole, all, &want, &from, &listed);
+            if (seen == 2) return listed;
+            if (seen == 1) looked = true, sub = SD_SHIFT - 8, split = from, from >>= sub;
+            else from = SD_BASE;
+        }
+        for (int level = looked ? 1 : 0;; ++level) {
+            if (!looked) clear_bins<MASS>();
             const auto bin = [&](float v) -> int {  // -1: not among those looked at
                 if (by_image) {
                     const unsigned o = ohi - ord_from_f32(v);
                     return o <= ohi - olo ? (int)(o >> sub) : -1;
                 }
                 const unsigned d = distance(v);
-                return (d >> in) == pre ? min(max((int)(d >> sub) - (int)from, 0), SBINS - 1) : -1;
+                const int b = (int)(d >> sub) - (int)from;
+                if (sub == SD_SHIFT) return min(max(b, 0), SBINS - 1);
+                return (d >> in) == pre && (unsigned)b < (unsigned)SBINS ? b : -1;
             };
-            each([&](const float (&v)[4], int i) {
+            if (!looked) each([&](const float (&v)[4], int i) {
                 int at[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) at[e] = kept(v[e], i + e) ? bin(v[e]) : -1;
@@ -527,7 +623,7 @@ struct Row {
                         }
                     }
             });
-            join_bins<MASS>();
+            if (!looked) join_bins<MASS>();
             const u64 m = MASS ? s.all_w[tid] : (u64)s.all_n[tid];
             if (MASS && level == 0) {
                 const u64 inc = block_scan(s, m);
@@ -536,7 +632,8 @@ struct Row {
                 *all = s.cut;
                 want = p <= 0.0f ? 1ull : max((u64)ceil((double)p * (double)*all), (u64)1);
             }
-            const int b = reach(m, base, want);
+            const int b = looked ? s.found : reach(m, base, want);
+            looked = false;
             if (b < 0) return 0;  // fewer entries than k: all are kept
             base = s.found_before;
             const unsigned n = s.all_n[b];
@@ -569,7 +666,7 @@ struct Row {
             if (!by_image && sub > 0 && (level > 0 || (b > 0 && b < SBINS - 1))) {
                 in = sub;
                 pre = from + (unsigned)b;
-                sub = sub == SD_SHIFT ? SD_SHIFT - 10 : 0;
+                sub = max(sub - 10, 0);
                 from = pre << (in - sub);
                 continue;
             }
@@ -650,6 +747,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     if (a.ctas > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");  // waited for before the first write to another CTA
 
     w.temp = temp;
+    w.split = 0;
     w.octaves = 64.0 / (0.693147180559945309417232 * (double)temp);
     w.per_t = fminf(1.0f / temp, 3e38f);
     w.scale_bits = (unsigned)(1023 + a.unit_bits) << 20;
@@ -746,8 +844,10 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     // ---- the draw ----
     unsigned count = 0;
     const auto keep = [&](float v, int i) { return w.kept(v, i); };
+    if (w.floor > w.thr) w.split = 0;  // min-p cuts higher: the sums above the other cut are of no use
     w.keep_from(max(w.thr, w.floor));
-    all = w.template sums<true>(keep, &count);
+    if (w.split != 0) all = w.template sums<true>([&](float v, int i) { return w.kept(v, i) && w.distance(v) >= w.split; }, &count);
+    else all = w.template sums<true>(keep, &count);
     count = __reduce_add_sync(0xffffffffu, count);
     if (lane == 0) s.warp_n[warp] = count;
     w.template walk<true>(keep, Row<T>::aim(u, all));
