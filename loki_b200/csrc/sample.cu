@@ -22,6 +22,7 @@
 //   bits of x, until at most 1,024 entries are left to be sorted, or all are equal and are cut by index.
 //   Then a pass sums the kept weights by warp and CTA, and the draw walks down those sums.
 #include <cfloat>
+#include <type_traits>
 
 #include "devops.cuh"
 
@@ -232,22 +233,26 @@ struct Row {
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
         const int lo = warp * wlen, hi = min(lo + wlen, len);
-#pragma unroll 1
-        for (int i = lo + lane * 4; i < hi; i += 128) {
-            float v[4];
-            if (i < a.cap) {  // whole: the stretch is padded with NaN
-                if constexpr (sizeof(T) == 4) {
-                    const float4 q = *reinterpret_cast<const float4 *>(data + i);
-                    v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-                } else {
-                    const uint2 q = *reinterpret_cast<const uint2 *>(data + i);
-                    const T *t = reinterpret_cast<const T *>(&q);
-                    v[0] = Elem<T>::get(t[0]), v[1] = Elem<T>::get(t[1]), v[2] = Elem<T>::get(t[2]), v[3] = Elem<T>::get(t[3]);
-                }
-            } else {
+        const bool groups = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+        using Group = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+        const auto fetch = [&](int i) {
+            Group q;
+            if (i < a.cap) return *reinterpret_cast<const Group *>(data + i);  // whole: the stretch is padded with NaN
+            if (groups && i + 4 <= hi) return *reinterpret_cast<const Group *>(x + i);
+            T *t = reinterpret_cast<T *>(&q);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = i + e < hi ? Elem<T>::get(x[i + e]) : CUDART_NAN_F;
-            }
+            for (int e = 0; e < 4; ++e) t[e] = i + e < hi ? x[i + e] : Elem<T>::put(CUDART_NAN_F);
+            return q;
+        };
+        int i = lo + lane * 4;
+        Group next = {};
+        if (i < hi) next = fetch(i);
+#pragma unroll 1
+        for (; i < hi; i += 128) {
+            const Group q = next;
+            if (i + 128 < hi) next = fetch(i + 128);  // under way while this one is worked on
+            const T *t = reinterpret_cast<const T *>(&q);
+            const float v[4] = {Elem<T>::get(t[0]), Elem<T>::get(t[1]), Elem<T>::get(t[2]), Elem<T>::get(t[3])};
             f(v, i);
         }
     }
