@@ -78,15 +78,11 @@ def _vector(t, what, types, index, n):
 
 
 _stream = torch._C._cuda_getCurrentRawStream
+_norm, _linear, _sample = lib.lk_rms_norm_i8, lib.lk_linear, lib.lk_sample
 _F32, _I32, _I64, _I8 = (torch.float32,), (torch.int32,), (torch.int64,), (torch.int8,)
 
 
 _new = torch.empty_strided
-
-
-def _codes(x, rows, dim):
-    """rows x dim int8 in rows of a multiple of 16 bytes, the padding zero: as linear reads them best."""
-    return x.new_zeros((rows, (dim + 15) // 16 * 16), dtype=torch.int8)[:, :dim]
 
 
 def rms_norm_i8(x, gain=None, *, residual=None, eps: float = 1e-6, out_codes=None, out_scales=None, out_sum=None):
@@ -94,7 +90,8 @@ def rms_norm_i8(x, gain=None, *, residual=None, eps: float = 1e-6, out_codes=Non
 
     ``codes * scales[:, None]`` is ``h / sqrt(mean(h ** 2) + eps) * gain`` with ``h = x + residual``,
     rounded to 8 bits; ``sum`` is ``h`` in the type of ``x`` (None without a residual).  ``gain`` is a
-    vector of any of the three floating types.  ``out_sum`` may be ``x`` or ``residual`` itself.
+    vector of any of the three floating types.  ``out_sum`` may be ``x`` or ``residual`` itself.  Codes that
+    are made here have rows on 16-byte boundaries, with whatever was there between them.
     """
     rows, dim, ldx, dev = _matrix(x, "x", _FLOATS)
     kind = x.dtype
@@ -113,16 +110,15 @@ def rms_norm_i8(x, gain=None, *, residual=None, eps: float = 1e-6, out_codes=Non
         s = out_sum.data_ptr()
     if out_codes is not None:
         ldc = _matrix(out_codes, "out_codes", _I8, dev, rows, dim)[2]
-    elif dim % 16 == 0:
-        out_codes, ldc = _new((rows, dim), (dim, 1), dtype=torch.int8, device=place), dim
-    else:
-        out_codes, ldc = _codes(x, rows, dim), (dim + 15) // 16 * 16
+    else:  # rows on 16-byte boundaries, as linear reads them best
+        ldc = (dim + 15) // 16 * 16
+        out_codes = _new((rows, dim), (ldc, 1), dtype=torch.int8, device=place)
     if out_scales is None:
         out_scales = _new((rows,), (1,), dtype=torch.float32, device=place)
         scales = out_scales.data_ptr()
     else:
         scales = _vector(out_scales, "out_scales", _F32, dev, rows)
-    st = lib.lk_rms_norm_i8(dev, _FLOATS[kind], rows, dim, x.data_ptr(), ldx, r, ldr, g, 0 if g is None else _FLOATS[gain.dtype], eps,
+    st = _norm(dev, _FLOATS[kind], rows, dim, x.data_ptr(), ldx, r, ldr, g, 0 if g is None else _FLOATS[gain.dtype], eps,
                             s, lds, out_codes.data_ptr(), ldc, scales, _stream(dev))
     if st:
         check(st)
@@ -138,8 +134,10 @@ def linear(a, w, *, a_scales=None, w_scales=None, bias=None, act: str = "none", 
     (float32 for int8).  ``out`` may be ``residual`` itself.  Rows on 16-byte boundaries run fastest.
     """
     m, k, lda, dev = _matrix(a, "a", _OPERANDS)
-    n, _, ldw, _ = _matrix(w, "w", (a.dtype,), dev, None, k)
-    if act not in ACTIVATIONS:
+    operands = a.dtype
+    n, _, ldw, _ = _matrix(w, "w", (operands,), dev, None, k)
+    activation = ACTIVATIONS.get(act)
+    if activation is None:
         _refuse(LK_EINVAL, f"act: one of {', '.join(ACTIVATIONS)}, not {act!r}")
     if out is not None:
         kind = out.dtype
@@ -152,20 +150,23 @@ def linear(a, w, *, a_scales=None, w_scales=None, bias=None, act: str = "none", 
     elif bias is not None:
         kind = bias.dtype
     else:
-        kind = torch.float32 if a.dtype == torch.int8 else a.dtype
-    if kind not in _FLOATS:
+        kind = torch.float32 if operands == torch.int8 else operands
+    result = _FLOATS.get(kind)
+    if result is None:
         _refuse(LK_EINVAL, f"out_dtype: {kind} is not supported here")
     r = ldr = 0
     if residual is not None:
         ldr = _matrix(residual, "residual", (kind,), dev, m, n)[2]
         r = residual.data_ptr()
-    sa, sw, b = _vector(a_scales, "a_scales", _F32, dev, m), _vector(w_scales, "w_scales", _F32, dev, n), _vector(bias, "bias", (kind,), dev, n)
+    sa = None if a_scales is None else _vector(a_scales, "a_scales", _F32, dev, m)
+    sw = None if w_scales is None else _vector(w_scales, "w_scales", _F32, dev, n)
+    b = None if bias is None else _vector(bias, "bias", (kind,), dev, n)
     if out is None:
         out, ldo = _new((m, n), (n, 1), dtype=kind, device=a.device), n
     else:
         ldo = _matrix(out, "out", (kind,), dev, m, n)[2]
-    st = lib.lk_linear(dev, _OPERANDS[a.dtype], m, n, k, a.data_ptr(), lda, sa, w.data_ptr(), ldw, sw, b, ACTIVATIONS[act], r, ldr,
-                       _FLOATS[kind], out.data_ptr(), ldo, _stream(dev))
+    st = _linear(dev, _OPERANDS[operands], m, n, k, a.data_ptr(), lda, sa, w.data_ptr(), ldw, sw, b, activation, r, ldr,
+                 result, out.data_ptr(), ldo, _stream(dev))
     if st:
         check(st)
     return out
@@ -203,7 +204,7 @@ def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, o
     place = scores.device
     ids = _new((rows,), (1,), dtype=torch.int64, device=place) if out_ids is None else out_ids
     probs, kept = _new((rows,), (1,), dtype=torch.float32, device=place), _new((rows,), (1,), dtype=torch.int32, device=place)
-    st = lib.lk_sample(dev, _FLOATS[scores.dtype], rows, vocab, scores.data_ptr(), ld, t, k, p, mp, up,
+    st = _sample(dev, _FLOATS[scores.dtype], rows, vocab, scores.data_ptr(), ld, t, k, p, mp, up,
                        _vector(ids, "out_ids", _I64, dev, rows), probs.data_ptr(), kept.data_ptr(), _stream(dev))
     if st:
         check(st)
