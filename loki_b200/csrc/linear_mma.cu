@@ -41,12 +41,24 @@ struct LinearTiles {
     int mt;              // rows of a per tile
     int stages, split;
     int slices;          // K slices of 128 bytes
-    int tiles_m;
+    int tiles_m, tiles_n, band;
     long long tiles;
     unsigned idesc;
     unsigned columns;    // tensor memory to allocate
     bool w_once;         // every row of w is read by one CTA only, and all of w is more than L2 would keep
 };
+
+// Place of tile t: bands of `band` tiles of w's rows, through which the tiles of a's rows run.  Where w is the smaller operand a
+// band as wide as w keeps it in L2 and reads a once: 8,192 x 4,096 x 4,096 bf16, sustained: 228 us with bands of 1, 216 of 8, 208 of
+// all 16.  Else bands of 8, which also serve an `a` that is too large to stay (4,096 x 8,192 x 4,096 int8: 102.5 us with bands of 1,
+// 103.7 of 8, 105.5 of 16).
+__device__ __forceinline__ void tile_at(const LinearTiles &g, long long t, int &tn, int &tm) {
+    const long long per = (long long)g.band * g.tiles_m;
+    const int band = (int)(t / per), r = (int)(t - band * per);
+    const int width = min(g.band, g.tiles_n - band * g.band);
+    tm = r / width;
+    tn = band * g.band + r - tm * width;
+}
 
 struct LinearShared {
     unsigned long long full[LMAX_STAGES], empty[LMAX_STAGES], acc_full[2], acc_empty[2], joined;
@@ -169,7 +181,9 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (joined) g_mbar_expect_tx(&ctl->joined, (unsigned)(g.mt * LW * 4));
         if (!PAIR && first < g.tiles) {  // the first stages are on their way while the CTA sets itself up
-            const int yw = (int)(first / g.tiles_m) * LW, ya = (int)(first % g.tiles_m) * g.mt;
+            int tn, tm;
+            tile_at(g, first, tn, tm);
+            const int yw = tn * LW, ya = tm * g.mt;
             for (int i = 0; i < early; ++i) {
                 g_mbar_expect_tx(&ctl->full[i], (unsigned)(LW_BYTES + a_bytes));
                 if (g.w_once) l_load_once(g_smem(sm_w + (size_t)i * LW_BYTES), &tm_w, (s0 + i) * LSLICE, yw, g_smem(&ctl->full[i]));
@@ -204,8 +218,10 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
         unsigned phase = 0;
         bool ok = true;
         for (long long t = first; ok && t < g.tiles; t += step) {
-            const int yw = (int)(t / g.tiles_m) * LW * CG + cta_of * LW;
-            const int ya = (int)(t % g.tiles_m) * g.mt + cta_of * (g.mt / CG);
+            int tn, tm;
+            tile_at(g, t, tn, tm);
+            const int yw = tn * LW * CG + cta_of * LW;
+            const int ya = tm * g.mt + cta_of * (g.mt / CG);
             for (int s = s0; s < s1; ++s) {
                 if (t == first && s - s0 < early) {
                     // already asked for.  Its stage must not be waited for either: it may have been used and freed by
@@ -266,8 +282,10 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
         int acc = 0;
         unsigned acc_phase = 0;
         for (long long t = first; t < g.tiles; t += step) {
-            const long long j = (t / g.tiles_m) * (LW * CG) + cta_of * LW + quad * 32 + lane;
-            const long long i0 = (t % g.tiles_m) * g.mt;
+            int tn, tm;
+            tile_at(g, t, tn, tm);
+            const long long j = (long long)tn * (LW * CG) + cta_of * LW + quad * 32 + lane;
+            const long long i0 = (long long)tm * g.mt;
             const bool live = j < p.n;
             const bool whole = i0 + g.mt <= p.m && (j | 31) < p.n;  // this warp's share lies inside the result
             const float sw = live ? scale_of(p.w_scales, j) : 0.0f;
@@ -365,7 +383,9 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
     // ------------------------------ joining the parts of K ------------------------------
     if (joined && warp >= 2) {  // one tile per cluster; this CTA's columns are mt / split of it
         const int own = g.mt / g.split, w = own >= 4 ? 4 : 2, items = own / w * LW;
-        const long long j0 = (first / g.tiles_m) * LW, i0 = (first % g.tiles_m) * g.mt + part_of * own;
+        int tn, tm;
+        tile_at(g, first, tn, tm);
+        const long long j0 = (long long)tn * LW, i0 = (long long)tm * g.mt + part_of * own;
         bool ok = true, waited = false;
         for (int e = tid - 64; e < items; e += LEPI_WARPS * 32) {  // one column of the result, w rows of it
             const int n = e % LW;
@@ -549,7 +569,11 @@ int linear_mma_launch(const LinearArgs &p, int dtype, int device, cudaStream_t s
     g.mt = plan.mt;
     g.split = plan.split;
     g.tiles_m = (int)((p.m + g.mt - 1) / g.mt);
-    g.tiles = g.tiles_m * ((p.n + LW * cg - 1) / (LW * cg));
+    g.tiles_n = (int)((p.n + LW * cg - 1) / (LW * cg));
+    g.tiles = (long long)g.tiles_m * g.tiles_n;
+    const long long a_bytes = p.m * p.k * eb, w_bytes = p.n * p.k * eb, keep = 48ll << 20;  // what stays in L2 beside the rest
+    if (a_bytes <= w_bytes) g.band = std::min(8, g.tiles_n);
+    else g.band = (int)std::min<long long>(g.tiles_n, std::max<long long>(16, keep / (LW * cg * p.k * eb)));
     g.stages = ring_stages(g.mt, cg, g.split);
     // 134 MB of w: 25.1 us with the hint, 26.4 without; 17 MB: no difference, and the next call may find it in L2
     g.w_once = g.tiles_m == 1 && p.n * p.k * eb > (64ll << 20);
