@@ -338,7 +338,8 @@ LK_API int lk_pca3(const float *vecs, int64_t n, int dim, int workers, int devic
  * each other.  The caller's current device is the same after the call as before it.  Strides (ld*)
  * are in ELEMENTS between the starts of consecutive rows; the elements of a row are contiguous.
  * Nothing outside the stated rows and columns is read or written.  Outputs must not overlap inputs
- * except where said.  A size of zero rows (or columns) is a call that does nothing. */
+ * except where said.  A size of zero rows (or columns) is a call that does nothing.  The first call of
+ * each function on a device asks the device for its limits: make it before a stream capture. */
 
 /* Root-mean-square norm of x (+ residual) to 8 bits, row by row:
  *   h = x + residual (float32);  y = h / sqrt(mean(h^2) + eps) * gain;

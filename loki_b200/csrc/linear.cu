@@ -102,6 +102,7 @@ extern "C" int lk_linear(int device, int dtype, int64_t m, int64_t n, int64_t k,
 extern "C" int lk_ops_status(int device) {
     DeviceScope scope;
     LK_TRY(scope.enter(device, "lk_ops_status"));
+    LK_CUDA(cudaDeviceSynchronize());  // streams that the legacy default stream does not wait for, too
     int linear = 0, norm = 0;
     LK_TRY(linear_failed(&linear));
     LK_TRY(norm_failed(&norm));

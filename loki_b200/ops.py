@@ -139,6 +139,9 @@ def linear(a, w, *, a_scales=None, w_scales=None, bias=None, act: str = "none", 
     activation = ACTIVATIONS.get(act)
     if activation is None:
         _refuse(LK_EINVAL, f"act: one of {', '.join(ACTIVATIONS)}, not {act!r}")
+    for t, what in ((out, "out"), (residual, "residual"), (bias, "bias")):
+        if t is not None and not isinstance(t, torch.Tensor):
+            _refuse(LK_EINVAL, f"{what}: a CUDA tensor is wanted")
     if out is not None:
         kind = out.dtype
         if out_dtype is not None and out_dtype != kind:

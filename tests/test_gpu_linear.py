@@ -167,7 +167,7 @@ def test_result_views_and_untouched_neighbours(ops, m, n, start):
         assert torch.all(left == 9.0)
 
 
-@pytest.mark.parametrize("m,n", [(1, 4096), (30, 520), (200, 264)])
+@pytest.mark.parametrize("m,n", [(1, 4096), (30, 520), (200, 264), (2100, 2050)])
 def test_residual_in_place(ops, m, n):
     g, a, w, sa, sw = operands(m, n, 256, torch.int8, 6)
     r = torch.randn(m, n, generator=g, device="cuda").bfloat16()

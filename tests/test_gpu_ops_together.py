@@ -123,3 +123,31 @@ def test_no_allocation_by_the_calls(ops, lk):
         ops.linear(out[0], s["table"], a_scales=out[1], w_scales=s["table_scales"], out=out[3])
     torch.cuda.synchronize()
     assert torch.cuda.mem_get_info()[0] == before
+
+
+def test_first_calls_of_new_sizes_in_a_capture(ops):
+    """Once a function has run on the device, any of its kernels may be met in a capture first."""
+    s = setting(rows=3, seed=8)
+    answer(ops, s)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(700, 2048, generator=g, device="cuda").half()
+    w = torch.randn(2100, 2048, generator=g, device="cuda").half()
+    u = torch.rand(700, generator=g, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        codes, scales, _ = ops.rms_norm_i8(x)
+        y = ops.linear(x, w, act="gelu")
+        ids, _, _ = ops.sample(y, u, top_p=0.9)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(codes, ops.rms_norm_i8(x)[0]) and torch.equal(y, ops.linear(x, w, act="gelu"))
+    assert torch.equal(ids, ops.sample(y, u, top_p=0.9)[0])
+
+
+def test_status_sees_side_streams(ops):
+    s = setting(rows=200, seed=2)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for _ in range(20):
+            out = answer(ops, s)
+    ops.check_device()  # waits for that stream too
+    assert same(out, answer(ops, s))

@@ -207,3 +207,45 @@ def test_refusals(ops, lk):
         a.update(kw)
         with pytest.raises(lk.LokiError):
             ops.sample(a.pop("scores"), a.pop("u"), **a)
+
+
+@pytest.mark.parametrize("vocab", [9000, 140001])
+@pytest.mark.parametrize("offset", [0.0, 1e4, -1e6])
+@pytest.mark.parametrize("spread", [1e-3, 0.1, 30.0, 1e4])
+def test_scores_of_any_size(ops, vocab, spread, offset):
+    """Nearly flat rows, rows that one score rules, scores far from zero (float32 then holds few distinct ones: many ties)."""
+    g, u, s = setting(5, int(vocab + spread * 7 + offset % 97), top_k=None, min_p=None)
+    x = scores(5, vocab, torch.float32, g, spread) + offset
+    verify(ops, x, u, **s)
+    verify(ops, x, u, top_p=s["top_p"], min_p=0.1 * s["top_p"])
+    verify(ops, x, u, temperature=s["temperature"], top_k=torch.randint(600, 5000, (5,), generator=g, device="cuda", dtype=torch.int32), top_p=s["top_p"])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_ties_across_a_long_row(ops, dtype):
+    """131,072 scores of a few hundred distinct values: every cut falls among thousands of equals, spread over all CTAs of the row."""
+    g = torch.Generator(device="cuda").manual_seed(40)
+    x = (torch.randint(-30, 5, (4, 131072), generator=g, device="cuda") / 8.0).to(dtype)
+    u = torch.rand(4, generator=g, device="cuda")
+    verify(ops, x, u, top_k=torch.tensor([700, 9000, 60000, 131071], dtype=torch.int32, device="cuda"))
+    verify(ops, x, u, top_p=torch.tensor([0.11, 0.37, 0.73, 0.991], device="cuda"))
+    verify(ops, x, u, top_k=torch.tensor([700, 9000, 60000, 131071], dtype=torch.int32, device="cuda"), top_p=torch.full((4,), 0.613, device="cuda"))
+
+
+def test_all_equal_in_a_long_row(ops):
+    x = torch.full((3, 200000), -2.5, device="cuda")
+    u = torch.tensor([0.0, 0.31234, 0.99], device="cuda")
+    n = torch.tensor([1000, 70000, 199999], device="cuda")
+    verify(ops, x, u, top_p=((n + 0.5) / 200000).float())
+    verify(ops, x, u, top_k=n.int())
+    verify(ops, x, u, temperature=torch.full((3,), 1e-20, device="cuda"))
+
+
+def test_temperatures_in_a_long_row(ops):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    t = torch.tensor([1e-38, 1e-6, 1e-2, 0.3, 5.0, 1e4, 1e30, 3e38], device="cuda")
+    x = scores(8, 70000, torch.float32, g)
+    u = torch.rand(8, generator=g, device="cuda")
+    verify(ops, x, u, temperature=t)
+    verify(ops, x, u, temperature=t, top_p=torch.full((8,), 0.777, device="cuda"))
+    verify(ops, x, u, temperature=t, min_p=torch.full((8,), 0.3, device="cuda"))
