@@ -262,7 +262,8 @@ struct NormRow {
             for (int t = 0; t < THREADS; t += 32) ss += s.sums[turn][t + lane];
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (lane == 0) a.scales[row] = (float)((double)__uint_as_float(top) * rsqrt(ss * a.per_dim + (double)a.eps)) / 127.0f;
+            if (lane == 0)  // a row of zeros: 0, whatever eps is
+                a.scales[row] = top != 0u ? (float)((double)__uint_as_float(top) * rsqrt(ss * a.per_dim + (double)a.eps)) / 127.0f : 0.0f;
         }
         return false;
     }

@@ -184,3 +184,50 @@ def test_refusals(ops, lk):
         a.update(kw)
         with pytest.raises(lk.LokiError):
             ops.rms_norm_i8(a.pop("x"), a.pop("gain"), **a)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,dim", [(592, 264), (700, 1024), (3001, 1032), (1500, 2048), (900, 2056), (2000, 4096), (600, 4104), (640, 8192), (600, 8200)])
+def test_many_wide_rows(ops, dtype, rows, dim):
+    """Enough rows to stream: every width of thread and stage."""
+    for residual in (False, True):
+        x, r, gain = make(rows, dim, dtype, dim + rows, residual)
+        verify(ops.rms_norm_i8(x, gain, residual=r, eps=1e-6), x, gain, r, 1e-6)
+    verify(ops.rms_norm_i8(x, gain.float(), eps=1e-6), x, gain.float(), None, 1e-6)
+    verify(ops.rms_norm_i8(x, eps=1e-6), x, None, None, 1e-6)
+
+
+@pytest.mark.parametrize("dim", [512, 4096])
+@pytest.mark.parametrize("into", ["new", "x", "residual"])
+def test_odd_rows_among_many(ops, dim, into):
+    """Zeros, NaN, infinities, and rows at the ends of the float range between ordinary ones; the sum in place or not."""
+    rows = 1900
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x = torch.randn(rows, dim, generator=g, device="cuda")
+    r = torch.randn(rows, dim, generator=g, device="cuda")
+    gain = 1 + torch.rand(dim, generator=g, device="cuda") * 7
+    kinds = torch.arange(rows, device="cuda") % 97
+    x[kinds == 3] = 0
+    r[kinds == 3] = 0
+    x[kinds == 10, dim // 3] = float("nan")
+    r[kinds == 20, 0] = float("inf")
+    x[kinds == 30, dim - 1] = float("-inf")
+    for kind, size in ((40, 1e38), (50, 1e-38), (60, 3e-41)):
+        x[kinds == kind] *= size
+        r[kinds == kind] *= size
+    x[kinds == 70] = torch.finfo(torch.float32).max
+    r[kinds == 70] = 0
+    a, b = x.clone(), r.clone()
+    out = None if into == "new" else (a if into == "x" else b)
+    codes, scales, total = ops.rms_norm_i8(a, gain, residual=b, eps=0.0, out_sum=out)
+    broken = (kinds == 10) | (kinds == 20) | (kinds == 30)
+    h = x + r
+    broken |= ~torch.isfinite(h).all(1)  # 1e38 times a normal number can pass the end of the range
+    assert torch.all(torch.isnan(scales[broken])) and torch.all(codes[broken] == 0)
+    verify((codes[~broken], scales[~broken], total[~broken]), x[~broken], gain, r[~broken], 0.0)
+    assert torch.equal(torch.nan_to_num(total[broken]), torch.nan_to_num(h[broken]))
+
+
+def test_no_wait_has_run_out(ops):
+    """All calls of this file: none gave up waiting for a copy."""
+    ops.check_device()
