@@ -562,7 +562,7 @@ int linear_mma_launch(const LinearArgs &p, int dtype, int device, cudaStream_t s
     const int eb = type_bytes(dtype), sms = sm_count(device);
     LinearTiles g;
     g.slices = (int)((p.k * eb + LSLICE - 1) / LSLICE);
-    const ClusterRoom *room;
+    const ClusterRoom *room = nullptr;
     LK_TRY(cluster_room(device, &room));
     const LinearPlan plan = linear_plan(p.m, p.n, g.slices, *room);
     const int cg = plan.pair ? 2 : 1;

@@ -58,7 +58,7 @@ struct alignas(16) SampleShared {
     unsigned all_n[SBINS];
     u64 list[SLIST];                           // this CTA's candidates
     u64 sorted[SLIST];                         // scratch of the sort
-    double octave[64];                         // 2^(j/64)
+    double octave[128][8];                     // 2^(j/128), eight times
     u64 warp_w[SWARPS];
     unsigned warp_n[SWARPS];
     u64 above_w[SWARPS];                       // look(): what lies above the cut's place, by warp
@@ -160,11 +160,11 @@ struct Row {
     float bottom;   // a score so far below it that it weighs nothing
     bool alone;     // nothing else weighs: it is +infinity, or T is that small
     double top_wide;
-    double octaves; // 64 / (T ln 2): a score in 64ths of an octave
+    double octaves; // 128 / (T ln 2): a score in 128ths of an octave
     double whole;   // 1.5 * 2^52 - N: adding it rounds to a whole number in the low word
-    unsigned scale_bits;  // exponent of 2^F
+    unsigned scale_bits;  // 2^F, to be added to an exponent
     float temp, per_t;  // T, 1 / T
-    unsigned split;     // 0, or the distance (its bits) above which look() has summed the weights by warp
+    float split;        // look() has summed the weights of what is above this by warp
     u64 floor;      // min_p: the lowest key that it keeps
     u64 thr;        // entries with a key at or above this are kept
     float thr_x;    // its score and its index
@@ -185,13 +185,24 @@ struct Row {
     }
     // NaN compares false; -infinity is below every threshold
     __device__ __forceinline__ bool kept(float v, int i) const { return v > thr_x || (v == thr_x && i <= thr_i); }
+    __device__ __forceinline__ void kept4(const float (&v)[4], int i, bool (&k)[4]) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k[e] = v[e] >= thr_x;
+        if (thr_i != 0x7fffffff) {  // a cut among equals
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = k[e] && !(v[e] == thr_x && i + e > thr_i);
+        }
+    }
     __device__ __forceinline__ float entry(int i) const { return Elem<T>::get(i < a.cap ? data[i] : x[i]); }
 
     // w * 2^F of a score, rounded, where others than the largest weigh.  Tang's scheme (ACM TOMS 15, 1989): with y = x / T / ln 2 *
-    // 64 = N + n + r, n whole, |r| <= 1/2, N the whole number next to the largest y:  w = 2^(n div 64) * 2^((n mod 64) / 64) *
-    // e^(r ln 2 / 64), the middle factor from a table, the last by its series to the fourth power (next term 4e-14).  All weights
-    // of a row share a factor within 2^(1/128) of 1 (the largest y is not whole), which no quotient of weights sees.  Roundings to
-    // whole numbers are done by adding constants, the power of two on the bits: conversions issue at an eighth of the rate.
+    // 128 = N + n + r, n whole, |r| <= 1/2, N the whole number next to the largest y:  w = 2^(n div 128) * 2^((n mod 128) / 128) *
+    // e^(r ln 2 / 128), the middle factor from a table, the last by its series to the third power (next term 2e-12 at most).
+    // All weights of a row share a factor within 2^(1/256) of 1 (the largest y is not whole), which no quotient of weights
+    // sees.  Roundings to whole numbers are done by adding constants, powers of two on the bits.
+    // Bound: the float64 pipe (2 clocks a warp and instruction; there are seven) and the table's banks: eight copies, a lane reads
+    // its own.  Clocks a warp and 32 scores, loads and loop apart: 25 with 1,024 entries, one copy and six float64
+    // instructions (17 of them the banks').
     // The result still carries the exponent bits of the last addition: kTag more than the weight.
     static constexpr u64 kTag = 0x4330000000000000ull;  // 2^52 as a float64
     __device__ __forceinline__ u64 tagged(float v) const {
@@ -199,13 +210,11 @@ struct Row {
         const double t = fma(x, octaves, whole);
         const double r = fma(x, octaves, whole - t);
         const int n = __double2loint(t);
-        constexpr double c = 0.693147180559945309417232 / 64;
-        double q = fma(r, c * c * c * c / 24, c * c * c / 6);
-        q = fma(r, q, c * c / 2);
-        q = fma(r, q, c);
-        q = fma(r, q, 1.0);
-        const double scale = __hiloint2double((int)(((unsigned)n * (1u << 14) + scale_bits) & 0xfff00000u), 0);
-        return (u64)__double_as_longlong(fma(s.octave[n & 63] * q, scale, 4503599627370496.0));  // + 2^52; w < 2^51
+        constexpr double c = 0.693147180559945309417232 / 128;
+        const double q = fma(r, fma(r, fma(r, c * c * c / 6, c * c / 2), c), 1.0);
+        const double f = s.octave[n & 127][lane & 7];
+        const double scaled = __hiloint2double(__double2hiint(f) + (int)(((unsigned)n * (1u << 13) & 0xfff00000u) + scale_bits), __double2loint(f));
+        return (u64)__double_as_longlong(fma(q, scaled, 4503599627370496.0));  // + 2^52; w < 2^51
     }
     __device__ __forceinline__ u64 weight(float v) const { return tagged(v) - kTag; }
     // The same for any row.
@@ -257,7 +266,7 @@ struct Row {
         }
     }
 
-    // Sum over the entries with keep(score, index) of their weights (MASS) or their number; warp_w keeps this CTA's warps'
+    // Sum over the entries that keep(scores, index, out) says of their weights (MASS) or their number; warp_w keeps this CTA's warps'
     // sums and slot_w the CTAs'.  *mine: how many of this thread's entries there are.
     template <bool MASS, typename K>
     __device__ __forceinline__ u64 sums(K keep, unsigned *mine) const {
@@ -265,11 +274,11 @@ struct Row {
         unsigned n = 0;
         each([&](const float (&v)[4], int i) {
             bool k[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) k[e] = keep(v[e], i + e);
+            keep(v, i, k);
             if (!(k[0] | k[1] | k[2] | k[3])) return;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) n += k[e];
+            for (int e = 0; e < 4; ++e)
+                if (k[e]) ++n;
             if (!MASS) return;
             if (alone) {
 #pragma unroll
@@ -278,14 +287,14 @@ struct Row {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const u64 m = tagged(v[e]);
-                    w += k[e] ? m : 0ull;
+                    if (k[e]) w += m;
                 }
             }
         });
         *mine = n;
         if (!MASS) w = n;
         else if (!alone) w -= n * kTag;
-        if (MASS && split != 0 && lane == 0) w += s.above_w[warp], *mine += s.above_n[warp];
+        if (MASS && split < CUDART_INF_F && lane == 0) w += s.above_w[warp], *mine += s.above_n[warp];
         w = warp_sum(w);
         __syncthreads();
         if (lane == 0) s.warp_w[warp] = w;
@@ -384,7 +393,7 @@ struct Row {
         unsigned lo = kNegInf + 1, hi = ord_from_f32(top);  // the largest score is always kept
         while (lo < hi) {
             const unsigned step = (hi - lo) / 32 + 1, mid = lo + min(lane * step, hi - lo);
-            const bool in = mid == hi || ((double)f32_from_ord(mid) - top_wide) * (octaves * (0.693147180559945309417232 / 64)) >= end;
+            const bool in = mid == hi || ((double)f32_from_ord(mid) - top_wide) * (octaves * (0.693147180559945309417232 / 128)) >= end;
             const int first = __ffs(__ballot_sync(0xffffffffu, in)) - 1;  // lanes ascend: the first that is kept, if any
             if (first < 0) lo += 31 * step + 1;
             else {
@@ -500,15 +509,18 @@ struct Row {
 
     // The first look of a cut by weight, at the price of one pass over the weights: the entries of each bin are counted, which
     // with the mean weight of a bin says to a thousandth where the cut is, and then one pass sums the kept weights of all, of what
-    // lies above the three bins around that place (by warp, for the draw), and bins those three finely.  The sums are exact:
-    // they show whether the cut is in there (1: found_before and all_n, all_w of the fine bins from `start` on are set), else the
-    // cut is made from the beginning (0).  2: there are at most SLIST entries down to there, and they are in the lists.
-    __device__ __forceinline__ int look(float p, bool whole_row, u64 *all, u64 *want, unsigned *start, int *listed) {
+    // lies above a stretch of scores around that place (by warp, for the draw; `split` is the stretch's upper end), and bins that
+    // stretch finely by the scores' images.  The sums are exact: they show whether the cut is in there (1: found, found_before
+    // and all_n, all_w of the fine bins of 2^sub images from ohi down are set), else the cut is made from the beginning (0).
+    // 2: there are at most SLIST entries down to there, and they are in the lists.
+    __device__ __forceinline__ int look(float p, bool whole_row, u64 *all, u64 *want, unsigned *olo, unsigned *ohi, int *sub, int *listed) {
         clear_bins<false>();
         each([&](const float (&v)[4], int i) {
+            bool k[4];
+            kept4(v, i, k);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (kept(v[e], i + e)) atomicAdd(&s.n[first_bin(distance(v[e]))], 1u);
+                if (k[e]) atomicAdd(&s.n[first_bin(distance(v[e]))], 1u);
         });
         join_bins<false>();
         const auto edge = [](int b) { return __uint_as_float((unsigned)(SD_BASE + b) << SD_SHIFT); };
@@ -524,37 +536,46 @@ struct Row {
         if (tid == ST - 1) s.found_w = upto;
         __syncthreads();
         const bool few = whole_row && s.found_w <= SLIST;
-        if (!few && b < 2) return 0;  // the first bin is not one of distances alike
-        const unsigned first = few ? 0u : (unsigned)(SD_BASE + b - 1) << SD_SHIFT, end = (unsigned)(SD_BASE + b + 2) << SD_SHIFT;
+        // the ends of the stretch, of the bins beside that one; how they are rounded does not matter
+        const float above_x = few || b == 0 ? CUDART_INF_F : (float)(top_wide - (double)edge(b - 1) * (double)temp);
+        const float below_x = fmaxf((float)(top_wide - (double)edge(b + 2) * (double)temp), -FLT_MAX);
+        *ohi = ord_from_f32(fminf(above_x, top));
+        *olo = ord_from_f32(below_x);
+        *sub = 0;
+        while (((*ohi - *olo) >> *sub) >= SBINS) ++*sub;
         __syncthreads();
         clear_bins<true>();
         u64 w_all = 0, w_above = 0;
-        unsigned n_above = 0;
+        unsigned n_all = 0, n_above = 0;
+        const float upper = few ? below_x : above_x;
         each([&](const float (&v)[4], int i) {
             bool k[4], in[4];
             u64 w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) k[e] = kept(v[e], i + e);
+            kept4(v, i, k);
             if (!(k[0] | k[1] | k[2] | k[3])) return;
-            weights(v, k, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = tagged(v[e]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const unsigned d = distance(v[e]);
-                const bool above = k[e] && d < (few ? end : first);
-                in[e] = k[e] && d < end && d >= first;
-                w_all += w[e];
-                w_above += above ? w[e] : 0ull;
-                n_above += above;
-                if (in[e] && !few) {
-                    const int at = (int)((d - first) >> (SD_SHIFT - 8));
-                    atomicAdd(&s.n[at], 1u);
-                    const unsigned l = (unsigned)w[e], old = atomicAdd(&s.lo[at], l);
-                    const unsigned h = (unsigned)(w[e] >> 32) + (old + l < l ? 1u : 0u);
-                    if (h) atomicAdd(&s.hi[at], h);
-                }
+                in[e] = k[e] && v[e] >= below_x && !(v[e] > above_x);
+                if (k[e]) w_all += w[e], ++n_all;
+                if (k[e] && (few ? v[e] >= upper : v[e] > upper)) w_above += w[e], ++n_above;
             }
             if (few) note(in, v, i);
+            else if (in[0] | in[1] | in[2] | in[3]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (in[e]) {
+                        const int at = (int)((*ohi - ord_from_f32(v[e])) >> *sub);
+                        atomicAdd(&s.n[at], 1u);
+                        const unsigned l = (unsigned)w[e], old = atomicAdd(&s.lo[at], l);
+                        const unsigned h = (unsigned)((w[e] - kTag) >> 32) + (old + l < l ? 1u : 0u);
+                        if (h) atomicAdd(&s.hi[at], h);
+                    }
+            }
         });
+        w_all -= n_all * kTag;
+        w_above -= n_above * kTag;
         w_all = warp_sum(w_all);
         w_above = warp_sum(w_above);
         n_above = __reduce_add_sync(0xffffffffu, n_above);
@@ -575,9 +596,9 @@ struct Row {
         for (int r = 0; r < a.ctas; ++r) *all += s.slot_w[r], above += s.slot_v[r];
         *want = p <= 0.0f ? 1ull : max((u64)ceil((double)p * (double)*all), (u64)1);
         sync();  // the slots may be written again
-        if (few) return above >= *want ? 2 : 0;
+        if (few) return above >= *want && *listed <= SLIST ? 2 : 0;
         if (above >= *want || reach(s.all_w[tid], above, *want) < 0) return 0;
-        *start = first;
+        split = above_x;
         return 1;
     }
 
@@ -593,10 +614,10 @@ struct Row {
         bool by_image = false, looked = false;
         if (MASS && !alone) {
             int listed;
-            const int seen = look(p, whole, all, &want, &from, &listed);
+            const int seen = look(p, whole, all, &want, &olo, &ohi, &sub, &listed);
             if (seen == 2) return listed;
-            if (seen == 1) looked = true, sub = SD_SHIFT - 8, split = from, from >>= sub;
-            else from = SD_BASE;
+            if (seen == 1) looked = by_image = true;
+            else sub = SD_SHIFT;
         }
         for (int level = looked ? 1 : 0;; ++level) {
             if (!looked) clear_bins<MASS>();
@@ -649,10 +670,16 @@ struct Row {
                 if (s.found_w <= SLIST && b < SBINS - 1) return (int)gather_to(b);
             }
             if (n <= SLIST) {
+                // (a bin of images is a stretch of scores)
+                const float from_x = by_image ? f32_from_ord(max(ohi - (((unsigned)b + 1u) << sub) + 1u, olo)) : -CUDART_INF_F;
+                const float to_x = by_image ? f32_from_ord(ohi - ((unsigned)b << sub)) : CUDART_INF_F;
                 each([&](const float (&v)[4], int i) {
                     bool among[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) among[e] = kept(v[e], i + e) && bin(v[e]) == b;
+                    for (int e = 0; e < 4; ++e) among[e] = v[e] >= from_x && v[e] <= to_x;
+                    if (!(among[0] | among[1] | among[2] | among[3])) return;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) among[e] = among[e] && kept(v[e], i + e) && bin(v[e]) == b;
                     note(among, v, i);
                 });
                 deliver();
@@ -709,7 +736,10 @@ struct Row {
                 if (need < n) {
                     const auto tie = [&](float v, int i) { return v == tied && kept(v, i); };
                     unsigned none;
-                    sums<false>(tie, &none);
+                    sums<false>([&](const float (&v)[4], int i, bool (&k)[4]) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) k[e] = tie(v[e], i + e);
+                    }, &none);
                     walk<false>(tie, need - 1);
                     if (tid == 0 && s.found >= 0)
                         for (int r = 0; r < a.ctas; ++r) s_put(s_at(&s.cut, r), key(tied, s.found));
@@ -748,14 +778,14 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     const float u = a.u[row];
     const bool bad = !(temp >= 0.0f) || p != p || least_in != least_in || u != u;
     if (temp == 0.0f) temp = 1.0f, k = 1;
-    if (tid < 64) s.octave[tid] = exp2(tid / 64.0);
+    s.octave[tid >> 3][tid & 7] = exp2((tid >> 3) / 128.0);  // as many as threads
     if (a.ctas > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");  // waited for before the first write to another CTA
 
     w.temp = temp;
-    w.split = 0;
-    w.octaves = 64.0 / (0.693147180559945309417232 * (double)temp);
+    w.split = CUDART_INF_F;
+    w.octaves = 128.0 / (0.693147180559945309417232 * (double)temp);
     w.per_t = fminf(1.0f / temp, 3e38f);
-    w.scale_bits = (unsigned)(1023 + a.unit_bits) << 20;
+    w.scale_bits = (unsigned)a.unit_bits << 20;
 
     // ---- the row comes in; its largest score ----
     const int held = min(w.len, a.cap);
@@ -849,10 +879,13 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     // ---- the draw ----
     unsigned count = 0;
     const auto keep = [&](float v, int i) { return w.kept(v, i); };
-    if (w.floor > w.thr) w.split = 0;  // min-p cuts higher: the sums above the other cut are of no use
+    if (w.floor > w.thr) w.split = CUDART_INF_F;  // min-p cuts higher: the sums above the other cut are of no use
     w.keep_from(max(w.thr, w.floor));
-    if (w.split != 0) all = w.template sums<true>([&](float v, int i) { return w.kept(v, i) && w.distance(v) >= w.split; }, &count);
-    else all = w.template sums<true>(keep, &count);
+    all = w.template sums<true>([&](const float (&v)[4], int i, bool (&k)[4]) {
+        w.kept4(v, i, k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k[e] = k[e] && !(v[e] > w.split);  // what lies above has been summed
+    }, &count);
     count = __reduce_add_sync(0xffffffffu, count);
     if (lane == 0) s.warp_n[warp] = count;
     w.template walk<true>(keep, Row<T>::aim(u, all));
