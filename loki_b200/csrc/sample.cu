@@ -530,15 +530,22 @@ struct Row {
         const u64 inc = block_scan(s, m);
         if (tid == ST - 1) s.cut = inc;
         __syncthreads();
-        const int b = reach(m, 0ull, max((u64)((double)fmaxf(p, 0.0f) * (double)s.cut), (u64)1));
+        const u64 near = max((u64)((double)fmaxf(p, 0.0f) * (double)s.cut), (u64)1);
+        const int b = reach(m, 0ull, near);
         if (b < 0 || b >= SBINS - 2) return 0;
         const u64 upto = block_scan(s, tid <= b + 1 ? s.all_n[tid] : 0u);
         if (tid == ST - 1) s.found_w = upto;
         __syncthreads();
         const bool few = whole_row && s.found_w <= SLIST;
-        // the ends of the stretch, of the bins beside that one; how they are rounded does not matter
-        const float above_x = few || b == 0 ? CUDART_INF_F : (float)(top_wide - (double)edge(b - 1) * (double)temp);
-        const float below_x = fmaxf((float)(top_wide - (double)edge(b + 2) * (double)temp), -FLT_MAX);
+        // the ends of the stretch, a bin to either side of the place (half a bin missed it now and then among bfloat16 scores, of
+        // which a bin holds one or two values); how they are rounded does not matter
+        const float d0 = b == 0 ? 0.0f : edge(b), d1 = edge(b + 1);
+        const float in_bin = (float)s.all_n[b] * ((__expf(-d0) - __expf(-d1)) / (d1 - d0)) * 1073741824.0f;
+        const float part = fminf(fmaxf((float)(near - s.found_before) / in_bin, 0.0f), 1.0f);
+        const float place = d0 + part * (d1 - d0), side = edge(b + 2) - edge(b + 1);
+        const float above_x = few || b == 0 ? CUDART_INF_F : (float)(top_wide - (double)(place - side) * (double)temp);
+        const float below_x = few ? fmaxf((float)(top_wide - (double)edge(b + 2) * (double)temp), -FLT_MAX)
+                                  : fmaxf((float)(top_wide - (double)((b == 0 ? d1 : place) + side) * (double)temp), -FLT_MAX);
         *ohi = ord_from_f32(fminf(above_x, top));
         *olo = ord_from_f32(below_x);
         *sub = 0;
