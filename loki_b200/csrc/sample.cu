@@ -46,6 +46,7 @@ constexpr int ST = 1024, SWARPS = ST / 32;
 constexpr int SBINS = 1024;                // one thread per bin
 constexpr int SLIST = 1024;                // one thread per candidate
 constexpr int SMAX_CTAS = 16;
+constexpr unsigned kSlack = 32;            // look(): entries to either side of an estimate
 constexpr int SD_SHIFT = 16, SD_BASE = (127 - 3) << 7;  // bins by d: exponent and 7 bits, from 2^-3 to 2^5
 using u64 = unsigned long long;
 // Measured, 64 x 131,072 and 8 x 1,000,000 scores: a CTA's time per entry over all passes, for its start and its sorts, and what
@@ -66,6 +67,8 @@ struct alignas(16) SampleShared {
     u64 slot_w[SMAX_CTAS], slot_v[SMAX_CTAS];  // one word from every CTA of the row
     unsigned slot_top[SMAX_CTAS], slot_n[SMAX_CTAS], slot_a[SMAX_CTAS], slot_b[SMAX_CTAS];
     unsigned noted;
+    unsigned n_before, n_upto, n_next;         // look(): entries above a bin, down to its end and to the next one's
+    int first, last;
     u64 cut;                                   // a decision of the first CTA, or of the one that holds an entry
     u64 found_w, found_before, floor;
     int found;
@@ -533,19 +536,32 @@ struct Row {
         const u64 near = max((u64)((double)fmaxf(p, 0.0f) * (double)s.cut), (u64)1);
         const int b = reach(m, 0ull, near);
         if (b < 0 || b >= SBINS - 2) return 0;
-        const u64 upto = block_scan(s, tid <= b + 1 ? s.all_n[tid] : 0u);
-        if (tid == ST - 1) s.found_w = upto;
+        // The estimate is off where few entries carry the weight, so the stretch goes on from the place's bin until it has kSlack
+        // more entries, down through bin `last` and up through bin `first` (0 or -1: from the largest score on).  When all that
+        // may be kept can be listed, the list ends with the last bin that keeps it to an eighth more than what the estimate says.
+        const unsigned n = s.all_n[tid], upto = (unsigned)block_scan(s, n), above_n = upto - n;
+        if (tid == 0) s.first = -1, s.last = SBINS - 2;
+        if (tid == b) s.n_before = above_n, s.n_upto = upto;
+        if (tid == b + 1) s.n_next = upto;
         __syncthreads();
-        const bool few = whole_row && s.found_w <= SLIST;
-        // the ends of the stretch, a bin to either side of the place (half a bin missed it now and then among bfloat16 scores, of
-        // which a bin holds one or two values); how they are rounded does not matter
+        const bool few = whole_row && s.n_next <= SLIST;
+        const unsigned down = few ? min(s.n_next + s.n_next / 8 + kSlack, (unsigned)SLIST) : s.n_upto + kSlack - 1;
+        if (upto > down && above_n <= down && tid <= SBINS - 2) s.last = few ? tid - 1 : tid;
+        if (s.n_before >= kSlack && above_n <= s.n_before - kSlack && upto > s.n_before - kSlack) s.first = tid;
+        __syncthreads();
+        const int first = s.first, last = s.last;
+        // the ends of the stretch; how they are rounded does not matter
         const float d0 = b == 0 ? 0.0f : edge(b), d1 = edge(b + 1);
         const float in_bin = (float)s.all_n[b] * ((__expf(-d0) - __expf(-d1)) / (d1 - d0)) * 1073741824.0f;
         const float part = fminf(fmaxf((float)(near - s.found_before) / in_bin, 0.0f), 1.0f);
         const float place = d0 + part * (d1 - d0), side = edge(b + 2) - edge(b + 1);
-        const float above_x = few || b == 0 ? CUDART_INF_F : (float)(top_wide - (double)(place - side) * (double)temp);
-        const float below_x = few ? fmaxf((float)(top_wide - (double)edge(b + 2) * (double)temp), -FLT_MAX)
-                                  : fmaxf((float)(top_wide - (double)((b == 0 ? d1 : place) + side) * (double)temp), -FLT_MAX);
+        const bool dense = s.all_n[b] >= 16 * kSlack;
+        const float above_d = dense && first == b - 1 ? place - side : edge(max(first, 0));
+        const float below_d = dense && last == b + 1 ? place + side : edge(last + 1);
+        const float above_x = few || first <= 0 ? CUDART_INF_F : (float)(top_wide - (double)above_d * (double)temp);
+        // (a list must not take in a value on the bin's edge, of which there may be hundreds)
+        const double below_wide = top_wide - (double)below_d * (few ? 1.0 - 1e-6 : 1.0) * (double)temp;
+        const float below_x = fmaxf(few ? __double2float_ru(below_wide) : (float)below_wide, -FLT_MAX);
         *ohi = ord_from_f32(fminf(above_x, top));
         *olo = ord_from_f32(below_x);
         *sub = 0;
