@@ -46,7 +46,7 @@ constexpr int ST = 1024, SWARPS = ST / 32;
 constexpr int SBINS = 1024;                // one thread per bin
 constexpr int SLIST = 1024;                // one thread per candidate
 constexpr int SMAX_CTAS = 16;
-constexpr unsigned kSlack = 32;            // look(): entries to either side of an estimate
+constexpr unsigned kSlack = 256;           // look(): entries to either side of an estimate
 constexpr int SD_SHIFT = 16, SD_BASE = (127 - 3) << 7;  // bins by d: exponent and 7 bits, from 2^-3 to 2^5
 using u64 = unsigned long long;
 // Measured, 64 x 131,072 and 8 x 1,000,000 scores: a CTA's time per entry over all passes, for its start and its sorts, and what
@@ -545,7 +545,7 @@ struct Row {
         if (tid == b + 1) s.n_next = upto;
         __syncthreads();
         const bool few = whole_row && s.n_next <= SLIST;
-        const unsigned down = few ? min(s.n_next + s.n_next / 8 + kSlack, (unsigned)SLIST) : s.n_upto + kSlack - 1;
+        const unsigned down = few ? min(s.n_next + s.n_next / 8 + 32, (unsigned)SLIST) : s.n_upto + kSlack - 1;
         if (upto > down && above_n <= down && tid <= SBINS - 2) s.last = few ? tid - 1 : tid;
         if (s.n_before >= kSlack && above_n <= s.n_before - kSlack && upto > s.n_before - kSlack) s.first = tid;
         __syncthreads();
@@ -555,7 +555,7 @@ struct Row {
         const float in_bin = (float)s.all_n[b] * ((__expf(-d0) - __expf(-d1)) / (d1 - d0)) * 1073741824.0f;
         const float part = fminf(fmaxf((float)(near - s.found_before) / in_bin, 0.0f), 1.0f);
         const float place = d0 + part * (d1 - d0), side = edge(b + 2) - edge(b + 1);
-        const bool dense = s.all_n[b] >= 16 * kSlack;
+        const bool dense = s.all_n[b] >= 2 * kSlack;
         const float above_d = dense && first == b - 1 ? place - side : edge(max(first, 0));
         const float below_d = dense && last == b + 1 ? place + side : edge(last + 1);
         const float above_x = few || first <= 0 ? CUDART_INF_F : (float)(top_wide - (double)above_d * (double)temp);
