@@ -3,9 +3,9 @@
 // Every filter keeps a prefix of the row's order (score descending, index ascending), so what is kept is
 // described by its last entry: a 64-bit ranking key (score image, ~index) at or above which entries are kept.
 // Weights w = exp((x - max) / T) are computed in float64 and summed as 64-bit integers, w * 2^F with vocab *
-// 2^F <= 2^63 and F <= 50: sums do not depend on their order (shared-memory atomics, warps, CTAs), the prefix
-// that a cut finds and the running sum that a draw walks agree to the last bit, and a border between two
-// entries is met to ~2^-F of the largest weight.
+// 2^F <= 2^63 and F <= 50: sums do not depend on their order (shared-memory atomics, warps, CTAs), and the prefix
+// that a cut finds and the running sum that a draw walks agree to the last bit.  A border between two entries is
+// off by the weights' error: 2^-(F+1) of the largest weight from the rounding, 2e-12 of the weight from the series.
 //
 // A cluster of CTAs owns a row.  Each loads one stretch of it into its shared memory (what does not fit is read
 // again from L2), so scores cross HBM once; every later pass runs over shared memory, and the CTAs
@@ -18,9 +18,14 @@
 //   hold top_p of the weight have that few entries.
 // * Many.  A cut by count or weight: entries fall into 1,024 bins by the distance d = (max - x) / T, 128 bins to a
 //   factor of two from 1/8 to 32 (the bits of d without the low ones: monotone in x, and fine where a softmax
-//   has its weight; few entries of a warp meet in one bin).  The bin in which the measure reaches its target is cut again by the next bits of d, then by the
-//   bits of x, until at most 1,024 entries are left to be sorted, or all are equal and are cut by index.
+//   has its weight; few entries of a warp meet in one bin).  The bin in which the measure reaches its target is
+//   cut again by the next bits of d, then by the bits of x, until at most 1,024 entries are left to be sorted, or all
+//   are equal and are cut by index.  A cut by weight first tries to do with one pass over the weights (look()).
 //   Then a pass sums the kept weights by warp and CTA, and the draw walks down those sums.
+//
+// Measured, 64 x 131,072 bf16 scores, a row cut by top-p alone, of 65 us: loading 5, counting into bins 10, the pass over the
+// weights 22 (of which the weights 8, the sum above the cut 3, the bins' atomics 3), gathering 5, sorting 4, the last sums
+// 6 to 12, the walk 2; the rest are meetings.
 #include <cfloat>
 #include <type_traits>
 

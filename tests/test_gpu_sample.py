@@ -249,3 +249,29 @@ def test_temperatures_in_a_long_row(ops):
     verify(ops, x, u, temperature=t)
     verify(ops, x, u, temperature=t, top_p=torch.full((8,), 0.777, device="cuda"))
     verify(ops, x, u, temperature=t, min_p=torch.full((8,), 0.3, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [20001, 131072])
+@pytest.mark.parametrize("p", [0.5, 0.8, 0.9, 0.95, 0.99, 0.999])
+def test_weight_on_few_entries(ops, dtype, vocab, p):
+    """Peaked rows: a cut's place cannot be told well from how many entries there are at which distance."""
+    g = torch.Generator(device="cuda").manual_seed(int(1000 * p) + vocab)
+    t = torch.tensor([0.3, 0.5, 0.8, 1.0] * 2, device="cuda")
+    verify(ops, scores(8, vocab, dtype, g, 3.0), torch.rand(8, generator=g, device="cuda"), temperature=t,
+           top_p=torch.full((8,), p, device="cuda"))
+
+
+@pytest.mark.parametrize("each", [20, 150, 700])
+@pytest.mark.parametrize("lowest", [1.0, 4.0, 9.0])
+def test_distances_at_the_ends_of_stretches(ops, each, lowest):
+    """Distances just past a 128th of an octave for the upper half of the row and just short of one for the lower: a mean
+    over each 128th is wrong in one direction above and in the other below."""
+    g = torch.Generator(device="cuda").manual_seed(each)
+    edges = torch.cat([2.0 ** e * (1 + torch.arange(128, device="cuda", dtype=torch.float64) / 128) for e in range(-3, 4)])
+    edges = edges[edges < lowest]
+    half = edges.numel() // 2
+    d = torch.cat([edges[:half] * (1 + 1e-4), edges[half:] * (1 - 1e-4)])
+    x = torch.cat([torch.zeros(1, device="cuda", dtype=torch.float64), -d.repeat(each)]).float()
+    x = torch.stack([x[torch.randperm(x.numel(), generator=g, device="cuda")] for _ in range(6)])
+    verify(ops, x, torch.rand(6, generator=g, device="cuda"), top_p=torch.tensor([0.05, 0.3, 0.501, 0.77, 0.96, 0.9991], device="cuda"))
