@@ -174,6 +174,7 @@ struct Row {
     unsigned scale_bits;  // 2^F, to be added to an exponent
     float temp, per_t;  // T, 1 / T
     float split;        // look() has summed the weights of what is above this by warp
+    bool summed;        // those sums have become the ones of all that is kept
     u64 floor;      // min_p: the lowest key that it keeps
     u64 thr;        // entries with a key at or above this are kept
     float thr_x;    // its score and its index
@@ -304,7 +305,10 @@ struct Row {
         if (!MASS) w = n;
         else if (!alone) w -= n * kTag;
         if (MASS && split < CUDART_INF_F && lane == 0) w += s.above_w[warp], *mine += s.above_n[warp];
-        w = warp_sum(w);
+        return join_sums(warp_sum(w));
+    }
+    // From the warps' sums: warp_w, slot_w, and the sum over the row.
+    __device__ __forceinline__ u64 join_sums(u64 w) const {
         __syncthreads();
         if (lane == 0) s.warp_w[warp] = w;
         __syncthreads();
@@ -522,7 +526,8 @@ struct Row {
     // lies above a stretch of scores around that place (by warp, for the draw; `split` is the stretch's upper end), and bins that
     // stretch finely by the scores' images.  The sums are exact: they show whether the cut is in there (1: found, found_before
     // and all_n, all_w of the fine bins of 2^sub images from ohi down are set), else the cut is made from the beginning (0).
-    // 2: there are at most SLIST entries down to there, and they are in the lists.
+    // 2: there are at most SLIST entries down to there, and they are in the lists.  3: min_p cuts higher, and all that it keeps has
+    // been summed by warp.
     __device__ __forceinline__ int look(float p, bool whole_row, u64 *all, u64 *want, unsigned *olo, unsigned *ohi, int *sub, int *listed) {
         clear_bins<false>();
         each([&](const float (&v)[4], int i) {
@@ -568,7 +573,9 @@ struct Row {
         const float above_x = few || first <= 0 ? CUDART_INF_F : (float)(top_wide - (double)above_d * (double)temp);
         // (a list must not take in a value on the bin's edge, of which there may be hundreds)
         const double below_wide = top_wide - (double)below_d * (few ? 1.0 - 1e-6 : 1.0) * (double)temp;
-        const float below_x = fmaxf(few ? __double2float_ru(below_wide) : (float)below_wide, -FLT_MAX);
+        // min_p cuts higher than that: it is enough that what it keeps weighs less than the target
+        const bool by_floor = !few && floor > thr && f32_from_ord(key_ord(floor)) > above_x;
+        const float below_x = by_floor ? CUDART_INF_F : fmaxf(few ? __double2float_ru(below_wide) : (float)below_wide, -FLT_MAX);
         *ohi = ord_from_f32(fminf(above_x, top));
         *olo = ord_from_f32(below_x);
         *sub = 0;
@@ -577,7 +584,8 @@ struct Row {
         clear_bins<true>();
         u64 w_all = 0, w_above = 0;
         unsigned n_all = 0, n_above = 0;
-        const float upper = few ? below_x : above_x;
+        const float upper = few ? below_x : by_floor ? f32_from_ord(key_ord(floor)) : above_x;
+        const bool equal_too = few || by_floor;
         each([&](const float (&v)[4], int i) {
             bool k[4], in[4];
             u64 w[4];
@@ -589,7 +597,7 @@ struct Row {
             for (int e = 0; e < 4; ++e) {
                 in[e] = k[e] && v[e] >= below_x && !(v[e] > above_x);
                 if (k[e]) w_all += w[e], ++n_all;
-                if (k[e] && (few ? v[e] >= upper : v[e] > upper)) w_above += w[e], ++n_above;
+                if (k[e] && (equal_too ? v[e] >= upper : v[e] > upper)) w_above += w[e], ++n_above;
             }
             if (few) note(in, v, i);
             else if (in[0] | in[1] | in[2] | in[3]) {
@@ -620,6 +628,7 @@ struct Row {
             }
         }
         if (few) *listed = (int)deliver();
+        else if (by_floor) sync();
         else join_bins<true>();
         u64 above = 0;
         *all = 0;
@@ -627,6 +636,7 @@ struct Row {
         *want = p <= 0.0f ? 1ull : max((u64)ceil((double)p * (double)*all), (u64)1);
         sync();  // the slots may be written again
         if (few) return above >= *want && *listed <= SLIST ? 2 : 0;
+        if (by_floor) return above < *want ? 3 : 0;
         if (above >= *want || reach(s.all_w[tid], above, *want) < 0) return 0;
         split = above_x;
         return 1;
@@ -642,10 +652,16 @@ struct Row {
         int in = 31, sub = SD_SHIFT;
         unsigned pre = 0, from = SD_BASE, olo = 0, ohi = 0;
         bool by_image = false, looked = false;
+        int seen = 0;
         if (MASS && !alone) {
             int listed;
-            const int seen = look(p, whole, all, &want, &olo, &ohi, &sub, &listed);
+            seen = look(p, whole, all, &want, &olo, &ohi, &sub, &listed);
             if (seen == 2) return listed;
+            if (seen == 3) {
+                keep_from(floor);
+                summed = true;
+                return 0;
+            }
             if (seen == 1) looked = by_image = true;
             else sub = SD_SHIFT;
         }
@@ -703,15 +719,30 @@ struct Row {
                 // (a bin of images is a stretch of scores)
                 const float from_x = by_image ? f32_from_ord(max(ohi - (((unsigned)b + 1u) << sub) + 1u, olo)) : -CUDART_INF_F;
                 const float to_x = by_image ? f32_from_ord(ohi - ((unsigned)b << sub)) : CUDART_INF_F;
+                // the look's bin: what the stretch has above it is added to the sums of what lies above the stretch
+                const bool direct = MASS && seen == 1 && level == 1;
+                const float end_x = direct ? split : to_x;
+                u64 w_in = 0;
+                unsigned n_in = 0;
                 each([&](const float (&v)[4], int i) {
                     bool among[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) among[e] = v[e] >= from_x && v[e] <= to_x;
+                    for (int e = 0; e < 4; ++e) among[e] = v[e] >= from_x && v[e] <= end_x;
                     if (!(among[0] | among[1] | among[2] | among[3])) return;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) among[e] = among[e] && kept(v[e], i + e) && bin(v[e]) == b;
+                    for (int e = 0; e < 4; ++e) {
+                        if (!among[e]) continue;
+                        const int at = kept(v[e], i + e) ? bin(v[e]) : -1;
+                        among[e] = at == b;
+                        if (direct && at >= 0 && at < b) w_in += weight(v[e]), ++n_in;
+                    }
                     note(among, v, i);
                 });
+                if (direct) {
+                    w_in = warp_sum(w_in);
+                    n_in = __reduce_add_sync(0xffffffffu, n_in);
+                    if (lane == 0) s.above_w[warp] += w_in, s.above_n[warp] += n_in;
+                }
                 deliver();
                 if (rank == 0) {
                     const u64 mine = block_sort(s, fetch(), (int)n);
@@ -722,6 +753,16 @@ struct Row {
                 }
                 sync();
                 keep_from(s.cut);
+                if (direct) {  // and of the bin what is kept
+                    if (tid < (int)s.slot_n[rank] && s.list[tid] >= s.cut) {
+                        const u64 k = s.list[tid];
+                        const int of = (int)(key_slot(k) - (unsigned)start) / wlen;
+                        atomicAdd(&s.above_w[of], weight(f32_from_ord(key_ord(k))));
+                        atomicAdd(&s.above_n[of], 1u);
+                    }
+                    __syncthreads();
+                    summed = true;
+                }
                 return 0;
             }
             // too many: the next bits of the distance, where the bin is one value of the bits above
@@ -813,6 +854,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
 
     w.temp = temp;
     w.split = CUDART_INF_F;
+    w.summed = false;
     w.octaves = 128.0 / (0.693147180559945309417232 * (double)temp);
     w.per_t = fminf(1.0f / temp, 3e38f);
     w.scale_bits = (unsigned)a.unit_bits << 20;
@@ -909,13 +951,17 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     // ---- the draw ----
     unsigned count = 0;
     const auto keep = [&](float v, int i) { return w.kept(v, i); };
-    if (w.floor > w.thr) w.split = CUDART_INF_F;  // min-p cuts higher: the sums above the other cut are of no use
+    if (w.floor > w.thr) w.split = CUDART_INF_F, w.summed = false;  // min-p cuts higher: the sums above the other cut are of no use
     w.keep_from(max(w.thr, w.floor));
-    all = w.template sums<true>([&](const float (&v)[4], int i, bool (&k)[4]) {
-        w.kept4(v, i, k);
+    if (w.summed) {
+        all = w.join_sums(s.above_w[warp]);
+        if (lane == 0) count = s.above_n[warp];
+    } else
+        all = w.template sums<true>([&](const float (&v)[4], int i, bool (&k)[4]) {
+            w.kept4(v, i, k);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) k[e] = k[e] && !(v[e] > w.split);  // what lies above has been summed
-    }, &count);
+            for (int e = 0; e < 4; ++e) k[e] = k[e] && !(v[e] > w.split);  // what lies above has been summed
+        }, &count);
     count = __reduce_add_sync(0xffffffffu, count);
     if (lane == 0) s.warp_n[warp] = count;
     w.template walk<true>(keep, Row<T>::aim(u, all));
