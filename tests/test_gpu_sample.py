@@ -275,3 +275,17 @@ def test_distances_at_the_ends_of_stretches(ops, each, lowest):
     x = torch.cat([torch.zeros(1, device="cuda", dtype=torch.float64), -d.repeat(each)]).float()
     x = torch.stack([x[torch.randperm(x.numel(), generator=g, device="cuda")] for _ in range(6)])
     verify(ops, x, torch.rand(6, generator=g, device="cuda"), top_p=torch.tensor([0.05, 0.3, 0.501, 0.77, 0.96, 0.9991], device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [30011, 200000])
+def test_min_p_above_and_below_the_cut(ops, dtype, vocab):
+    """Both filters with weight in them, min-p from far above the top-p's cut to far below it."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x, u = scores(10, vocab, dtype, g, 1.5), torch.rand(10, generator=g, device="cuda")
+    least = torch.logspace(-4, -0.3, 10, device="cuda")
+    k = torch.randint(2000, vocab, (10,), generator=g, device="cuda", dtype=torch.int32)
+    for p in (0.2, 0.6, 0.95):
+        verify(ops, x, u, top_p=torch.full((10,), p, device="cuda"), min_p=least)
+        verify(ops, x, u, top_k=k, top_p=torch.full((10,), p, device="cuda"), min_p=least)
+        verify(ops, x, u, top_k=torch.full_like(k, 700), top_p=torch.full((10,), p, device="cuda"), min_p=least)
