@@ -3,7 +3,7 @@
 // Every filter keeps a prefix of the row's order (score descending, index ascending), so what is kept is
 // described by its last entry: a 64-bit ranking key (score image, ~index) at or above which entries are kept.
 // Weights w = exp((x - max) / T) are computed in float64 and summed as 64-bit integers, w * 2^F with vocab *
-// 2^F <= 2^63 and F <= 50: sums do not depend on their order (shared-memory atomics, warps, CTAs), and the prefix
+// 2^F <= 2^62 and F <= 49: sums do not depend on their order (shared-memory atomics, warps, CTAs), and the prefix
 // that a cut finds and the running sum that a draw walks agree to the last bit.  A border between two entries is
 // off by the weights' error: 2^-(F+1) of the largest weight from the rounding, 2e-12 of the weight from the series.
 //
@@ -213,9 +213,11 @@ struct Row {
     // Bound: the float64 pipe (2 clocks a warp and instruction; there are seven) and the table's banks: eight copies, a lane reads
     // its own.  Clocks a warp and 32 scores, loads and loop apart: 25 with 1,024 entries, one copy and six float64
     // instructions (17 of them the banks').
-    // The result still carries the exponent bits of the last addition: kTag more than the weight.
-    static constexpr u64 kTag = 0x4330000000000000ull;  // 2^52 as a float64
-    __device__ __forceinline__ u64 tagged(float v) const {
+    // plus() returns 2^52 + w * 2^F, a whole number below 2^53.  A thread's sum of weights stays below 2^53 too, so it can be taken in
+    // float64 without rounding (one instruction instead of two, and in a pipe with room): of n entries a thread has n / 1,024 and 5
+    // at most, F + log2 n <= 62 and F <= 49.
+    static constexpr double kOne = 4503599627370496.0;  // 2^52
+    __device__ __forceinline__ double plus(float v) const {
         const double x = (double)fmaxf(v, bottom);
         const double t = fma(x, octaves, whole);
         const double r = fma(x, octaves, whole - t);
@@ -224,9 +226,10 @@ struct Row {
         const double q = fma(r, fma(r, fma(r, c * c * c / 6, c * c / 2), c), 1.0);
         const double f = s.octave[n & 127][lane & 7];
         const double scaled = __hiloint2double(__double2hiint(f) + (int)(((unsigned)n * (1u << 13) & 0xfff00000u) + scale_bits), __double2loint(f));
-        return (u64)__double_as_longlong(fma(q, scaled, 4503599627370496.0));  // + 2^52; w < 2^51
+        return fma(q, scaled, kOne);
     }
-    __device__ __forceinline__ u64 weight(float v) const { return tagged(v) - kTag; }
+    static __device__ __forceinline__ u64 whole_of(double p) { return (u64)__double_as_longlong(p) - 0x4330000000000000ull; }
+    __device__ __forceinline__ u64 weight(float v) const { return whole_of(plus(v)); }
     // The same for any row.
     __device__ __forceinline__ u64 weight_of(float v) const {
         if (alone) return v == top ? 1ull << a.unit_bits : 0ull;
@@ -280,8 +283,9 @@ struct Row {
     // sums and slot_w the CTAs'.  *mine: how many of this thread's entries there are.
     template <bool MASS, typename K>
     __device__ __forceinline__ u64 sums(K keep, unsigned *mine) const {
-        u64 w = 0;
+        double sum = 0.0;
         unsigned n = 0;
+        const double one = (double)(1ull << a.unit_bits);
         each([&](const float (&v)[4], int i) {
             bool k[4];
             keep(v, i, k);
@@ -292,18 +296,18 @@ struct Row {
             if (!MASS) return;
             if (alone) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w += k[e] && v[e] == top ? 1ull << a.unit_bits : 0ull;
+                for (int e = 0; e < 4; ++e)
+                    if (k[e] && v[e] == top) sum += one;
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const u64 m = tagged(v[e]);
-                    if (k[e]) w += m;
+                    const double w = plus(v[e]) - kOne;
+                    if (k[e]) sum += w;
                 }
             }
         });
         *mine = n;
-        if (!MASS) w = n;
-        else if (!alone) w -= n * kTag;
+        u64 w = MASS ? (u64)sum : (u64)n;
         if (MASS && split < CUDART_INF_F && lane == 0) w += s.above_w[warp], *mine += s.above_n[warp];
         return join_sums(warp_sum(w));
     }
@@ -582,22 +586,22 @@ struct Row {
         while (((*ohi - *olo) >> *sub) >= SBINS) ++*sub;
         __syncthreads();
         clear_bins<true>();
-        u64 w_all = 0, w_above = 0;
-        unsigned n_all = 0, n_above = 0;
-        const float upper = few ? below_x : by_floor ? f32_from_ord(key_ord(floor)) : above_x;
-        const bool equal_too = few || by_floor;
+        double sum_all = 0.0, sum_above = 0.0;
+        unsigned n_above = 0;
+        const float upper = few ? nextafterf(below_x, -CUDART_INF_F) : by_floor ? nextafterf(f32_from_ord(key_ord(floor)), -CUDART_INF_F) : above_x;
         each([&](const float (&v)[4], int i) {
             bool k[4], in[4];
-            u64 w[4];
+            double w[4];
             kept4(v, i, k);
             if (!(k[0] | k[1] | k[2] | k[3])) return;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = tagged(v[e]);
+            for (int e = 0; e < 4; ++e) w[e] = plus(v[e]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 in[e] = k[e] && v[e] >= below_x && !(v[e] > above_x);
-                if (k[e]) w_all += w[e], ++n_all;
-                if (k[e] && (equal_too ? v[e] >= upper : v[e] > upper)) w_above += w[e], ++n_above;
+                const double whole = w[e] - kOne;
+                if (k[e]) sum_all += whole;
+                if (k[e] && v[e] > upper) sum_above += whole, ++n_above;
             }
             if (few) note(in, v, i);
             else if (in[0] | in[1] | in[2] | in[3]) {
@@ -606,16 +610,14 @@ struct Row {
                     if (in[e]) {
                         const int at = (int)((*ohi - ord_from_f32(v[e])) >> *sub);
                         atomicAdd(&s.n[at], 1u);
-                        const unsigned l = (unsigned)w[e], old = atomicAdd(&s.lo[at], l);
-                        const unsigned h = (unsigned)((w[e] - kTag) >> 32) + (old + l < l ? 1u : 0u);
+                        const u64 m = whole_of(w[e]);
+                        const unsigned l = (unsigned)m, old = atomicAdd(&s.lo[at], l);
+                        const unsigned h = (unsigned)(m >> 32) + (old + l < l ? 1u : 0u);
                         if (h) atomicAdd(&s.hi[at], h);
                     }
             }
         });
-        w_all -= n_all * kTag;
-        w_above -= n_above * kTag;
-        w_all = warp_sum(w_all);
-        w_above = warp_sum(w_above);
+        u64 w_all = warp_sum((u64)sum_all), w_above = warp_sum((u64)sum_above);
         n_above = __reduce_add_sync(0xffffffffu, n_above);
         if (lane == 0) s.warp_w[warp] = w_all, s.above_w[warp] = w_above, s.above_n[warp] = n_above;
         __syncthreads();
@@ -909,7 +911,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     w.top = f32_from_ord(top);
     w.top_wide = (double)w.top;
     w.whole = 6755399441055744.0 - rint(w.top_wide * w.octaves);
-    // 62 octaves down a weight rounds to 0 (F <= 50).  Where the next lower float32 is further down than that, nothing but the
+    // 62 octaves down a weight rounds to 0 (F <= 49).  Where the next lower float32 is further down than that, nothing but the
     // largest score weighs; else `bottom` is 62 to 124 octaves down, or the lowest score there is.
     const double deep = 62.0 * 0.693147180559945309417232 * (double)temp;
     w.alone = !(w.top_wide - (double)nextafterf(w.top, -CUDART_INF_F) < deep);  // true for +infinity
@@ -1054,7 +1056,7 @@ extern "C" int lk_sample(int device, int dtype, int64_t rows, int64_t vocab, con
     int bits = 0;  // 2^bits >= vocab
     while ((1ll << bits) < vocab) ++bits;
     SampleArgs a = {d_logits, ld, (int)vocab, 1, 0, 0, d_temperature, d_top_p, d_min_p, d_u, d_top_k,
-                    reinterpret_cast<long long *>(d_ids), d_probs, d_kept, std::min(63 - bits, 50)};
+                    reinterpret_cast<long long *>(d_ids), d_probs, d_kept, std::min(62 - bits, 49)};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == LK_F32) return sample_launch<float>(a, rows, device, st);
     if (dtype == LK_F16) return sample_launch<__half>(a, rows, device, st);
