@@ -65,7 +65,7 @@ struct alignas(16) SampleShared {
     unsigned all_n[SBINS];
     u64 list[SLIST];                           // this CTA's candidates
     u64 sorted[SLIST];                         // scratch of the sort
-    double octave[128][8];                     // 2^(j/128), eight times
+    double octave[128][8];                     // 2^(F + j/128), eight times
     u64 warp_w[SWARPS];
     unsigned warp_n[SWARPS];
     u64 above_w[SWARPS];                       // look(): what lies above the cut's place, by warp
@@ -171,7 +171,6 @@ struct Row {
     double top_wide;
     double octaves; // 128 / (T ln 2): a score in 128ths of an octave
     double whole;   // 1.5 * 2^52 - N: adding it rounds to a whole number in the low word
-    unsigned scale_bits;  // 2^F, to be added to an exponent
     float temp, per_t;  // T, 1 / T
     float split;        // look() has summed the weights of what is above this by warp
     bool summed;        // those sums have become the ones of all that is kept
@@ -225,7 +224,7 @@ struct Row {
         constexpr double c = 0.693147180559945309417232 / 128;
         const double q = fma(r, fma(r, fma(r, c * c * c / 6, c * c / 2), c), 1.0);
         const double f = s.octave[n & 127][lane & 7];
-        const double scaled = __hiloint2double(__double2hiint(f) + (int)(((unsigned)n * (1u << 13) & 0xfff00000u) + scale_bits), __double2loint(f));
+        const double scaled = __hiloint2double(__double2hiint(f) + (int)(((unsigned)n & ~127u) << 13), __double2loint(f));
         return fma(q, scaled, kOne);
     }
     static __device__ __forceinline__ u64 whole_of(double p) { return (u64)__double_as_longlong(p) - 0x4330000000000000ull; }
@@ -539,7 +538,7 @@ struct Row {
             kept4(v, i, k);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (k[e]) atomicAdd(&s.n[first_bin(distance(v[e]))], 1u);
+                if (k[e]) atomicAdd(&s.n[first_bin(__float_as_uint((top - v[e]) * per_t))], 1u);  // distance(), as top is finite
         });
         join_bins<false>();
         const auto edge = [](int b) { return __uint_as_float((unsigned)(SD_BASE + b) << SD_SHIFT); };
@@ -598,10 +597,11 @@ struct Row {
             for (int e = 0; e < 4; ++e) w[e] = plus(v[e]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                in[e] = k[e] && v[e] >= below_x && !(v[e] > above_x);
                 const double whole = w[e] - kOne;
+                const bool over = k[e] && v[e] > upper;
                 if (k[e]) sum_all += whole;
-                if (k[e] && v[e] > upper) sum_above += whole, ++n_above;
+                if (over) sum_above += whole, ++n_above;
+                in[e] = few ? over : k[e] && !over && v[e] >= below_x;
             }
             if (few) note(in, v, i);
             else if (in[0] | in[1] | in[2] | in[3]) {
@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     const float u = a.u[row];
     const bool bad = !(temp >= 0.0f) || p != p || least_in != least_in || u != u;
     if (temp == 0.0f) temp = 1.0f, k = 1;
-    s.octave[tid >> 3][tid & 7] = exp2((tid >> 3) / 128.0);  // as many as threads
+    s.octave[tid >> 3][tid & 7] = exp2((tid >> 3) / 128.0) * (double)(1ull << a.unit_bits);  // as many as threads
     if (a.ctas > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");  // waited for before the first write to another CTA
 
     w.temp = temp;
@@ -859,7 +859,6 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     w.summed = false;
     w.octaves = 128.0 / (0.693147180559945309417232 * (double)temp);
     w.per_t = fminf(1.0f / temp, 3e38f);
-    w.scale_bits = (unsigned)a.unit_bits << 20;
 
     // ---- the row comes in; its largest score ----
     const int held = min(w.len, a.cap);
