@@ -862,7 +862,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
 
     // ---- the row comes in; its largest score ----
     const int held = min(w.len, a.cap);
-    unsigned own = 0;  // the largest that this thread has seen
+    float largest = -CUDART_INF_F;  // that this thread has seen; fmaxf passes over NaN
     int done = 0;
     if ((reinterpret_cast<uintptr_t>(w.x) & 15) == 0) {
         const int vecs = held / PER;
@@ -879,16 +879,17 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
                     reinterpret_cast<uint4 *>(w.data)[v0 + e * ST] = q[e];
                     const T *t = reinterpret_cast<const T *>(&q[e]);
 #pragma unroll
-                    for (int i = 0; i < PER; ++i) own = max(own, ord_from_f32(Elem<T>::get(t[i])));
+                    for (int i = 0; i < PER; ++i) largest = fmaxf(largest, Elem<T>::get(t[i]));
                 }
         }
     }
     for (int i = done + tid; i < w.len; i += ST) {
         const T t = w.x[i];
         if (i < held) w.data[i] = t;
-        own = max(own, ord_from_f32(Elem<T>::get(t)));
+        largest = fmaxf(largest, Elem<T>::get(t));
     }
     for (int i = held + tid; i < (int)round_up(held, PER); i += ST) w.data[i] = Elem<T>::put(CUDART_NAN_F);
+    const unsigned own = ord_from_f32(largest);
     unsigned top = __reduce_max_sync(0xffffffffu, own);
     if (lane == 0) s.warp_n[warp] = top;
     __syncthreads();
