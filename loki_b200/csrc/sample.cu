@@ -865,7 +865,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     float largest = -CUDART_INF_F;  // that this thread has seen; fmaxf passes over NaN
     int done = 0;
     if ((reinterpret_cast<uintptr_t>(w.x) & 15) == 0) {
-        const int vecs = held / PER;
+        const int vecs = w.len / PER, to_keep = held / PER;  // (cap is a multiple of PER)
         done = vecs * PER;
         constexpr int U = 4;
         for (int v0 = tid; v0 < vecs; v0 += ST * U) {
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
 #pragma unroll
             for (int e = 0; e < U; ++e)
                 if (v0 + e * ST < vecs) {
-                    reinterpret_cast<uint4 *>(w.data)[v0 + e * ST] = q[e];
+                    if (v0 + e * ST < to_keep) reinterpret_cast<uint4 *>(w.data)[v0 + e * ST] = q[e];
                     const T *t = reinterpret_cast<const T *>(&q[e]);
 #pragma unroll
                     for (int i = 0; i < PER; ++i) largest = fmaxf(largest, Elem<T>::get(t[i]));
