@@ -54,10 +54,10 @@ constexpr int SMAX_CTAS = 16;
 constexpr unsigned kSlack = 256;           // look(): entries to either side of an estimate
 constexpr int SD_SHIFT = 16, SD_BASE = (127 - 3) << 7;  // bins by d: exponent and 7 bits, from 2^-3 to 2^5
 using u64 = unsigned long long;
-// Measured with a top-p alone, 1 to 512 rows of 4,096 to 1,000,000 scores: a CTA's time per entry over all passes (one that its
-// shared memory does not hold costs it twice), for its start and its sorts, and what the meetings of a cluster add, and of
-// one of more than eight.  A row with a small top-k costs less per entry, but the host does not see the filters.
-constexpr double SAMPLE_ENTRY_NS = 0.7, SAMPLE_CTA_NS = 15000.0, SAMPLE_MEET_NS = 8000.0, SAMPLE_WIDE_NS = 6000.0;
+// Measured with a top-p alone, 1 to 512 rows of 4,096 to 1,000,000 scores: a CTA's time per entry over all passes, and for one that
+// its shared memory does not hold, its start and its sorts, and what the meetings of a cluster add, and of one of more
+// than eight.  A row with a small top-k costs less per entry, but the host does not see the filters.
+constexpr double SAMPLE_ENTRY_NS = 0.5, SAMPLE_AWAY_NS = 0.15, SAMPLE_CTA_NS = 15000.0, SAMPLE_MEET_NS = 8000.0, SAMPLE_WIDE_NS = 6000.0;
 
 struct alignas(16) SampleShared {
     unsigned lo[SBINS], hi[SBINS], n[SBINS];   // this CTA's bins: weights (two words), entries
@@ -1012,17 +1012,15 @@ static int sample_launch(SampleArgs a, long long rows, int device, cudaStream_t 
         asked[device] = true;
     }
     // The number of CTAs to a row that finishes first: clusters run in waves, a CTA's time is its entries (those past what
-    // its shared memory holds cost more) and its meetings.  Of two that finish within 5 % of one another the larger cluster: rows
-    // differ, and short ones make room sooner (128 x 131,072 bf16: 123 us with one CTA to a row, with two 127 us if all rows
-    // are cut by a top-p alone and 102 us if every other one has a top-k).
+    // its shared memory holds cost more) and its meetings.
     double least = 1e300;
     for (int c = 1; c <= SMAX_CTAS; ++c) {
         if (c > 1 && fit[device][c] < 1) continue;
         const double waves = (double)((rows + std::max(fit[device][c], 1) - 1) / std::max(fit[device][c], 1));
         const double seg = (double)((a.vocab + c - 1) / c);
-        const double cost = waves * (SAMPLE_ENTRY_NS * (seg + std::max(0.0, seg - kHold)) + (c > 1 ? SAMPLE_MEET_NS : 0.0) +
+        const double cost = waves * (SAMPLE_ENTRY_NS * seg + SAMPLE_AWAY_NS * std::max(0.0, seg - kHold) + (c > 1 ? SAMPLE_MEET_NS : 0.0) +
                                      (c > 8 ? SAMPLE_WIDE_NS : 0.0) + SAMPLE_CTA_NS);
-        if (cost < 1.05 * least) least = std::min(least, cost), a.ctas = c;
+        if (cost < least) least = cost, a.ctas = c;
     }
     a.seg = (int)round_up((a.vocab + a.ctas - 1) / a.ctas, 64);
     a.cap = std::min(a.seg, kHold);
