@@ -21,11 +21,10 @@
 //   has its weight; few entries of a warp meet in one bin).  The bin in which the measure reaches its target is
 //   cut again by the next bits of d, then by the bits of x, until at most 1,024 entries are left to be sorted, or all
 //   are equal and are cut by index.  A cut by weight first tries to do with one pass over the weights (look()).
-//   Then a pass sums the kept weights by warp and CTA, and the draw walks down those sums.
+//   Then a pass sums the kept weights by warp and CTA, if that look has not, and the draw walks down those sums.
 //
-// Measured, 64 x 131,072 bf16 scores, a row cut by top-p alone, of 65 us: loading 5, counting into bins 10, the pass over the
-// weights 22 (of which the weights 8, the sum above the cut 3, the bins' atomics 3), gathering 5, sorting 4, the last sums
-// 6 to 12, the walk 2; the rest are meetings.
+// Measured, 64 x 131,072 bf16 scores, rows cut by top-p 0.9 alone, of 56 us: loading 3, the maximum 2.5, counting into bins 9, the
+// pass over the weights with what is joined after it 21.5, gathering 5.5, sorting 5, the walk 2.5; the rest are meetings.
 #include <cfloat>
 #include <type_traits>
 
@@ -209,9 +208,8 @@ struct Row {
     // e^(r ln 2 / 128), the middle factor from a table, the last by its series to the third power (next term 2e-12 at most).
     // All weights of a row share a factor within 2^(1/256) of 1 (the largest y is not whole), which no quotient of weights
     // sees.  Roundings to whole numbers are done by adding constants, powers of two on the bits.
-    // Bound: the float64 pipe (2 clocks a warp and instruction; there are seven) and the table's banks: eight copies, a lane reads
-    // its own.  Clocks a warp and 32 scores, loads and loop apart: 25 with 1,024 entries, one copy and six float64
-    // instructions (17 of them the banks').
+    // Bound: issue slots, like the passes that call it (about 8 of the 20 us of a pass over 65,536 scores).  The table has eight
+    // copies, so that the lanes of a warp seldom meet in a bank (with one copy of 1,024 entries the banks took 17 clocks a warp).
     // plus() returns 2^52 + w * 2^F, a whole number below 2^53.  A thread's sum of weights stays below 2^53 too, so it can be taken in
     // float64 without rounding (one instruction instead of two, and in a pipe with room): of n entries a thread has n / 1,024 and 5
     // at most, F + log2 n <= 62 and F <= 49.
