@@ -7,6 +7,8 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <atomic>
+#include <mutex>
 #include <string>
 
 #include "../../include/lokiscan.h"
@@ -101,10 +103,36 @@ class DeviceScope {
 // rms_norm.cu: whether one of its bounded waits ran out on the current device since the last call; waits for the device.
 int norm_failed(int *out);
 
+// What a device is asked, or told, once: the first call on it does so, and calls that come meanwhile wait until it is done.  What
+// went wrong is tried again by the next call.
+class OncePerDevice {
+  public:
+    template <typename F>
+    int run(int device, F ask) {
+        if (done_[device].load(std::memory_order_acquire)) return 0;
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (done_[device].load(std::memory_order_relaxed)) return 0;
+        LK_TRY(ask());
+        done_[device].store(true, std::memory_order_release);
+        return 0;
+    }
+
+  private:
+    std::mutex mutex_;
+    std::atomic<bool> done_[kMaxDevices] = {};
+};
+
 // SMs of a device, asked once.
 inline int sm_count(int device) {
+    static OncePerDevice once;
     static int known[kMaxDevices];
-    if (known[device] == 0 && cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess) known[device] = 148;
+    once.run(device, [&] {
+        if (cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+            cudaGetLastError();
+            known[device] = 148;
+        }
+        return 0;
+    });
     return known[device];
 }
 

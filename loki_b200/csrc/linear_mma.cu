@@ -463,13 +463,13 @@ struct LinearPlan {
 
 // Clusters of 2, 4 and 8 full CTAs that run at the same time on a device, asked once.
 struct ClusterRoom {
-    bool known;
     int of[9];
 };
 static int cluster_room(int device, const ClusterRoom **out) {
+    static OncePerDevice once;
     static ClusterRoom rooms[kMaxDevices];
     ClusterRoom &r = rooms[device];
-    if (!r.known) {
+    LK_TRY(once.run(device, [&] {
         const void *f = (const void *)k_linear_mma<false, true, float>;
         LK_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
         cudaLaunchAttribute attr[1];
@@ -487,8 +487,8 @@ static int cluster_room(int device, const ClusterRoom **out) {
             if (cudaOccupancyMaxActiveClusters(&r.of[c], f, &cfg) != cudaSuccess) r.of[c] = 0;
         }
         cudaGetLastError();
-        r.known = true;
-    }
+        return 0;
+    }));
     *out = &r;
     return 0;
 }
@@ -530,12 +530,12 @@ static LinearPlan linear_plan(long long m, long long n, int slices, const Cluste
 template <bool PAIR, bool I8, typename Out>
 static int mma_launch(const CUtensorMap &tw, const CUtensorMap &ta, const LinearArgs &p, const LinearTiles &g, int device, int sms, cudaStream_t st) {
     constexpr int CG = PAIR ? 2 : 1;
-    static bool sized[kMaxDevices];
+    static OncePerDevice sized;
     const size_t smem = (size_t)g.stages * (LW_BYTES + g.mt / CG * LSLICE) + (g.split > 1 ? g.mt * LW * 4 : 0) + sizeof(LinearShared) + 1024;
-    if (!sized[device]) {
+    LK_TRY(sized.run(device, [] {
         LK_CUDA(cudaFuncSetAttribute((const void *)k_linear_mma<PAIR, I8, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-        sized[device] = true;
-    }
+        return 0;
+    }));
     const int per = PAIR ? 2 : g.split;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(std::min<long long>(g.tiles, std::max(1, sms / per)) * per));

@@ -368,16 +368,16 @@ static int row_launch(const NormArgs &a, cudaStream_t st) {
 // Rows in a CTA's ring, and the launch; -1 where the other kernel is the one to take.
 template <typename T, int THREADS, int V, int PER_SM>
 static int rows_launch(NormArgs a, int device, cudaStream_t st) {
-    static bool sized[kMaxDevices];
+    static OncePerDevice sized;
     const int fixed = (int)(sizeof(NormShared<THREADS>) + 127) / 128 * 128;
     const int part = (a.row_bytes + 127) / 128 * 128;
     a.stage_bytes = 2 * part;
     a.stages = std::min((227 * 1024 / PER_SM - 1024 - fixed) / a.stage_bytes, 16);
     if (a.stages < 2) return -1;
-    if (!sized[device]) {
+    LK_TRY(sized.run(device, [] {
         LK_CUDA(cudaFuncSetAttribute((const void *)k_norm_rows<T, THREADS, V, PER_SM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-        sized[device] = true;
-    }
+        return 0;
+    }));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)std::min<long long>(a.rows, (long long)sm_count(device) * PER_SM));
     cfg.blockDim = dim3(THREADS);

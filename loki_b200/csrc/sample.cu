@@ -988,7 +988,7 @@ template <typename T>
 static int sample_launch(SampleArgs a, long long rows, int device, cudaStream_t st) {
     constexpr size_t kSmem = 227 * 1024;
     constexpr int kHold = (int)((kSmem - sizeof(SampleShared)) / sizeof(T)) & ~63;
-    static bool asked[kMaxDevices];
+    static OncePerDevice asked;
     static int fit[kMaxDevices][SMAX_CTAS + 1];  // clusters of so many full CTAs that run at the same time
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
@@ -997,7 +997,7 @@ static int sample_launch(SampleArgs a, long long rows, int device, cudaStream_t 
     cfg.blockDim = dim3(ST);
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (!asked[device]) {
+    LK_TRY(asked.run(device, [&] {
         LK_CUDA(cudaFuncSetAttribute((const void *)k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
         LK_CUDA(cudaFuncSetAttribute((const void *)k_sample<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         cfg.dynamicSmemBytes = kSmem;
@@ -1007,8 +1007,8 @@ static int sample_launch(SampleArgs a, long long rows, int device, cudaStream_t 
             if (cudaOccupancyMaxActiveClusters(&fit[device][c], k_sample<T>, &cfg) != cudaSuccess) fit[device][c] = 0;
         }
         cudaGetLastError();
-        asked[device] = true;
-    }
+        return 0;
+    }));
     // The number of CTAs to a row that finishes first: clusters run in waves, a CTA's time is its entries (those past what
     // its shared memory holds cost more) and its meetings.
     double least = 1e300;

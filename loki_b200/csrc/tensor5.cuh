@@ -130,18 +130,15 @@ typedef CUresult (*encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, vo
                               const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 inline encode_fn get_encode() {
-    static encode_fn fn = nullptr;
-    static bool tried = false;
-    if (!tried) {
-        tried = true;
+    static const encode_fn fn = [] {  // looked up once; threads that come meanwhile wait for it
         void *p = nullptr;
         cudaDriverEntryPointQueryResult qr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess &&
-            qr == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<encode_fn>(p);
-        else
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) != cudaSuccess) {
             cudaGetLastError();
-    }
+            return encode_fn(nullptr);
+        }
+        return qr == cudaDriverEntryPointSuccess ? reinterpret_cast<encode_fn>(p) : encode_fn(nullptr);
+    }();
     return fn;
 }
 
