@@ -87,8 +87,8 @@ __device__ __forceinline__ float top3(float a, float b, float c) {
     return d;
 }
 
-// A row that is not finite, or where h * g leaves the comfortable range of float32 (overflow, or max|p| below 2^-100): all of
-// it again in float64, from memory.
+// A row that is not finite, or where h * g leaves the comfortable range of float32 (overflow, or max|p| below 2^-100, 0 among that
+// where h is not all 0): all of it again in float64, from memory.
 template <typename T, int THREADS>
 __device__ void slow_row(const NormArgs &a, NormShared<THREADS> &s, long long row) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -120,7 +120,7 @@ __device__ void slow_row(const NormArgs &a, NormShared<THREADS> &s, long long ro
     float scale = (float)(top * rsqrt(ss * a.per_dim + (double)a.eps) / 127.0);
     const bool good = top < CUDART_INF && ss < CUDART_INF && scale < CUDART_INF_F;
     if (!good) scale = CUDART_NAN_F;
-    const double step = good ? 127.0 / top : 0.0;
+    const double step = good && top > 0.0 ? 127.0 / top : 0.0;  // gains of zero alone: codes and scale are 0
 #pragma unroll 1
     for (int e = tid; e < a.dim; e += THREADS) {
         const float h = sum_of(e);  // before its place is written: x or r may be where the sum goes
@@ -211,6 +211,7 @@ struct NormRow {
             for (int i = 0; i < 8; i += 2) high = top3(high, p[v][i], p[v][i + 1]);
         }
         unsigned top = __float_as_uint(high) & 0x7fffffffu;
+        if (top == 0u && ss + ss2 != 0.0) top = 1u;  // h is not zero here: a product that underflowed, or a gain of zero (slow_row tells)
         top = __reduce_max_sync(0xffffffffu, top);
         s.sums[turn][tid] = ss + ss2;
         if (lane == 0) s.tops[turn][warp] = top;
