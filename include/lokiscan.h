@@ -353,8 +353,10 @@ LK_API int lk_pca3(const float *vecs, int64_t n, int dim, int workers, int devic
  *   d_sum       NULL, or h rounded to dtype (the residual of the next layer); may be the same
  *               array as d_x or d_residual, with the same stride
  *   d_codes     rows x dim int8;  d_scales rows floats
- * A row of zeros gets scale 0 and codes 0; a row in which h or y has a NaN or an infinity gets
- * scale NaN and codes 0, so that whatever is computed from it is NaN. */
+ * Only h and the results are held in float32: products with the gain and y may leave its range.
+ * A row of zeros gets scale 0 and codes 0; a row in which h or the gain has a NaN or an infinity, or
+ * whose scale is past float32's range, gets scale NaN and codes 0, so that whatever is computed from it
+ * is NaN. */
 #define LK_NORM_MAX_DIM 32768
 LK_API int lk_rms_norm_i8(int device, int dtype, int64_t rows, int dim, const void *d_x, int64_t ldx,
                           const void *d_residual, int64_t ldr, const void *d_gain, int gain_dtype, float eps,

@@ -257,14 +257,29 @@ struct NormRow {
         }
         // The sum of squares and the row's square root: one warp's work, another one's for the next row, under the others' way
         // to the next meeting.
+        bool over = false;
         if (warp == round % WARPS) {
             ss = 0.0;
 #pragma unroll
             for (int t = 0; t < THREADS; t += 32) ss += s.sums[turn][t + lane];
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (lane == 0)  // a row of zeros: 0, whatever eps is
-                a.scales[row] = top != 0u ? (float)((double)__uint_as_float(top) * rsqrt(ss * a.per_dim + (double)a.eps)) / 127.0f : 0.0f;
+            if (lane == 0) {
+                float scale = 0.0f;  // a row of zeros: 0, whatever eps is
+                if (top != 0u) {
+                    const double y = (double)__uint_as_float(top) * rsqrt(ss * a.per_dim + (double)a.eps);
+                    scale = (float)y / 127.0f;
+                    if (!(scale < CUDART_INF_F)) scale = (float)(y / 127.0);  // a y past float32 may have a scale that is not
+                    if (!(scale < CUDART_INF_F)) scale = CUDART_NAN_F, over = true;
+                }
+                a.scales[row] = scale;
+            }
+        }
+        // A scale is at most sqrt(dim) / 127 times the largest gain, so only a row wider than 127^2 can have one past float32.
+        if constexpr (THREADS * V * 8 > 127 * 127) {
+            if (__syncthreads_or(over))
+#pragma unroll 1
+                for (int e = tid; e < a.dim; e += THREADS) codes[e] = 0;
         }
         return false;
     }

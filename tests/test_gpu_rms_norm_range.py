@@ -28,7 +28,7 @@ def verify(got, h, gain, eps):
     over = s > MAX * (1 + E / 2)
     assert torch.all(torch.isnan(scales[over])) and torch.all(codes[over] == 0)
     fine = ~over
-    assert (codes[fine].double() - q[fine]).abs().max() <= 0.5 + 127 * 5 * E
+    assert torch.all((codes[fine].double() - q[fine]).abs() <= 0.5 + 127 * 5 * E)
     assert torch.all((scales[fine].double() - s[fine]).abs() <= s[fine] * 4 * E + TINY)
     return over
 
@@ -71,3 +71,24 @@ def test_gains_of_zero(ops, rows, dim):
     gain[dim // 2] = 1e-30
     x *= 1e-20
     verify(ops.rms_norm_i8(x, gain, eps=0.0), x, gain, 0.0)
+
+
+@pytest.mark.parametrize("rows", [1, 700])
+@pytest.mark.parametrize("dim", [20, 500, 4096, 8192, 16129, 16384, 20001, 32768])
+@pytest.mark.parametrize("gains", [1e30, 3e37, 3e38])
+def test_values_past_the_range_whose_scale_is_not(ops, rows, dim, gains):
+    """One element carries its row, so that the largest y is sqrt(dim) * gain: past float32, where the scale, a 127th of it, is a
+    float32 up to dim = 16,129, and beyond with smaller gains.  Where it is not, the row is not finite."""
+    if rows > 1 and dim > 8192:
+        rows = 5
+    h = torch.zeros(rows, dim, device="cuda")
+    at = torch.arange(rows, device="cuda") * 7 % dim
+    h[torch.arange(rows, device="cuda"), at] = 1.0
+    h[:, 3] += 0.125
+    gain = torch.full((dim,), gains, device="cuda")
+    over = verify(ops.rms_norm_i8(h, gain, eps=0.0), h, gain, 0.0)
+    assert bool(over.all()) == (gains == 3e38 and dim > 20001)
+    x = torch.zeros_like(h)
+    got = ops.rms_norm_i8(x, gain, residual=h, eps=0.0, out_sum=x)
+    verify(got, h, gain, 0.0)
+    assert torch.equal(x, h)
