@@ -399,7 +399,8 @@ LK_API int lk_ops_status(int device);
  * weight (at least one); of those the ones with w >= min_p (at least the first).  The draw is the
  * first INDEX (ascending) at which the running sum of the kept weights exceeds u times their sum.
  * Weights are summed as 64-bit integers (fixed point), so the result does not depend on an order
- * of additions: the same inputs give the same draw on every call.
+ * of additions: the same inputs give the same draw on every call.  A running sum is off by at most
+ * 2^-26 of the row's weight (2^-27 up to 2^18 scores), the probability by that and its own rounding.
  *   dtype          LK_F32 / LK_F16 / LK_BF16: type of the rows x vocab scores
  *   vocab          at most LK_SAMPLE_MAX_VOCAB
  *   d_temperature  rows floats, NULL = 1 everywhere; 0 = the largest score (top_k = 1)

@@ -2,10 +2,14 @@
 //
 // Every filter keeps a prefix of the row's order (score descending, index ascending), so what is kept is
 // described by its last entry: a 64-bit ranking key (score image, ~index) at or above which entries are kept.
-// Weights w = exp((x - max) / T) are computed in float64 and summed as 64-bit integers, w * 2^F with vocab *
-// 2^F <= 2^62 and F <= 49: sums do not depend on their order (shared-memory atomics, warps, CTAs), and the prefix
-// that a cut finds and the running sum that a draw walks agree to the last bit.  A border between two entries is
-// off by the weights' error: 2^-(F+1) of the largest weight from the rounding, 2e-12 of the weight from the series.
+// Weights w = exp((x - max) / T) are computed in float64 and summed as 64-bit integers, w * 2^F with sums below
+// 2^62 and F <= 49: sums do not depend on their order (shared-memory atomics, warps, CTAs), and the prefix
+// that a cut finds and the running sum that a draw walks agree to the last bit.  Each weight is rounded by 2^-(F+1) of the
+// largest at most, and by 2e-12 of itself (the series), so that a sum over n entries is off by n 2^-(F+1) at most, all in one direction
+// where their scores are equal.  Up to 2^18 entries F follows from their number, n 2^F <= 2^62: 2^-27 of the largest weight.
+// A longer row takes F from a bound on its own sum, the largest weight that each thread has seen times its entries: where F is 49
+// the sums of 2^24 entries are off by 2^-26 of the largest weight, elsewhere by 2^-28 of the sum, as the bound is at most 1,040 times that.
+// 2^-26 of the row's weight is a quarter of the step between two neighbouring values of u below 1.
 //
 // A cluster of CTAs owns a row.  Each loads one stretch of it into its shared memory (what does not fit is read
 // again from L2), so scores cross HBM once; every later pass runs over shared memory, and the CTAs
@@ -42,7 +46,7 @@ struct SampleArgs {
     long long *ids;
     float *probs;
     int *kept;
-    int unit_bits;  // F
+    int unit_bits;  // F, or what it is at least
 };
 
 constexpr unsigned kNegInf = 0x007fffffu;  // image of -infinity; NaN (0) is below it
@@ -50,6 +54,7 @@ constexpr int ST = 1024, SWARPS = ST / 32;
 constexpr int SBINS = 1024;                // one thread per bin
 constexpr int SLIST = 1024;                // one thread per candidate
 constexpr int SMAX_CTAS = 16;
+constexpr int kWide = 1 << 18;             // rows longer than this choose F by their scores (WIDE)
 constexpr unsigned kSlack = 256;           // look(): entries to either side of an estimate
 constexpr int SD_SHIFT = 16, SD_BASE = (127 - 3) << 7;  // bins by d: exponent and 7 bits, from 2^-3 to 2^5
 using u64 = unsigned long long;
@@ -156,7 +161,7 @@ __device__ __noinline__ u64 block_scan(SampleShared &s, u64 v) {
 }
 
 // One row, as the CTAs of its cluster see it.
-template <typename T>
+template <typename T, bool WIDE>
 struct Row {
     static constexpr int PER = 16 / sizeof(T);  // entries of a 16-byte group
     const SampleArgs &a;
@@ -171,6 +176,7 @@ struct Row {
     double octaves; // 128 / (T ln 2): a score in 128ths of an octave
     double whole;   // 1.5 * 2^52 - N: adding it rounds to a whole number in the low word
     float temp, per_t;  // T, 1 / T
+    int unit_bits;      // F
     float split;        // look() has summed the weights of what is above this by warp
     bool summed;        // those sums have become the ones of all that is kept
     u64 floor;      // min_p: the lowest key that it keeps
@@ -203,6 +209,10 @@ struct Row {
     }
     __device__ __forceinline__ float entry(int i) const { return Elem<T>::get(i < a.cap ? data[i] : x[i]); }
 
+    // About exp((v - than) / T), for v <= than.
+    __device__ __forceinline__ float lighter(float v, float than) const {
+        return v == than ? 1.0f : than == CUDART_INF_F ? 0.0f : exp2f((float)(((double)v - (double)than) * octaves / 128.0));
+    }
     // w * 2^F of a score, rounded, where others than the largest weigh.  Tang's scheme (ACM TOMS 15, 1989): with y = x / T / ln 2 *
     // 128 = N + n + r, n whole, |r| <= 1/2, N the whole number next to the largest y:  w = 2^(n div 128) * 2^((n mod 128) / 128) *
     // e^(r ln 2 / 128), the middle factor from a table, the last by its series to the third power (next term 2e-12 at most).
@@ -210,9 +220,7 @@ struct Row {
     // sees.  Roundings to whole numbers are done by adding constants, powers of two on the bits.
     // Bound: issue slots, like the passes that call it (about 8 of the 20 us of a pass over 65,536 scores).  The table has eight
     // copies, so that the lanes of a warp seldom meet in a bank (with one copy of 1,024 entries the banks took 17 clocks a warp).
-    // plus() returns 2^52 + w * 2^F, a whole number below 2^53.  A thread's sum of weights stays below 2^53 too, so it can be taken in
-    // float64 without rounding (one instruction instead of two, and in a pipe with room): of n entries a thread has n / 1,024 and 5
-    // at most, F + log2 n <= 62 and F <= 49.
+    // plus() returns 2^52 + w * 2^F, a whole number below 2^53.
     static constexpr double kOne = 4503599627370496.0;  // 2^52
     __device__ __forceinline__ double plus(float v) const {
         const double x = (double)fmaxf(v, bottom);
@@ -229,14 +237,14 @@ struct Row {
     __device__ __forceinline__ u64 weight(float v) const { return whole_of(plus(v)); }
     // The same for any row.
     __device__ __forceinline__ u64 weight_of(float v) const {
-        if (alone) return v == top ? 1ull << a.unit_bits : 0ull;
+        if (alone) return v == top ? 1ull << unit_bits : 0ull;
         return weight(v);
     }
     // Of four scores; those that are not kept weigh nothing.
     __device__ __forceinline__ void weights(const float (&v)[4], const bool (&k)[4], u64 (&w)[4]) const {
         if (alone) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = k[e] && v[e] == top ? 1ull << a.unit_bits : 0ull;
+            for (int e = 0; e < 4; ++e) w[e] = k[e] && v[e] == top ? 1ull << unit_bits : 0ull;
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -276,13 +284,26 @@ struct Row {
         }
     }
 
+    // A thread's sum of weights.  It can be taken in float64 without rounding (one instruction instead of two, and in a pipe with room)
+    // where it stays below 2^53: of n entries a thread has n / 1,024 and 5 at most, F + log2 n <= 62 and F <= 49.  A WIDE row's F says
+    // nothing about a thread's share: there four weights, below 2^52, are added in float64 and then to a whole number.
+    struct Sum {
+        double part = WIDE ? kOne : 0.0;
+        u64 before = 0;
+        __device__ __forceinline__ void add(double w) { part += w; }
+        __device__ __forceinline__ void next() {  // behind four weights at most
+            if constexpr (WIDE) before += whole_of(part), part = kOne;
+        }
+        __device__ __forceinline__ u64 get() const { return WIDE ? before : (u64)part; }
+    };
+
     // Sum over the entries that keep(scores, index, out) says of their weights (MASS) or their number; warp_w keeps this CTA's warps'
     // sums and slot_w the CTAs'.  *mine: how many of this thread's entries there are.
     template <bool MASS, typename K>
     __device__ __forceinline__ u64 sums(K keep, unsigned *mine) const {
-        double sum = 0.0;
+        Sum sum;
         unsigned n = 0;
-        const double one = (double)(1ull << a.unit_bits);
+        const double one = (double)(1ull << unit_bits);
         each([&](const float (&v)[4], int i) {
             bool k[4];
             keep(v, i, k);
@@ -294,17 +315,18 @@ struct Row {
             if (alone) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (k[e] && v[e] == top) sum += one;
+                    if (k[e] && v[e] == top) sum.add(one);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const double w = plus(v[e]) - kOne;
-                    if (k[e]) sum += w;
+                    if (k[e]) sum.add(w);
                 }
             }
+            sum.next();
         });
         *mine = n;
-        u64 w = MASS ? (u64)sum : (u64)n;
+        u64 w = MASS ? sum.get() : (u64)n;
         if (MASS && split < CUDART_INF_F && lane == 0) w += s.above_w[warp], *mine += s.above_n[warp];
         return join_sums(warp_sum(w));
     }
@@ -583,7 +605,7 @@ struct Row {
         while (((*ohi - *olo) >> *sub) >= SBINS) ++*sub;
         __syncthreads();
         clear_bins<true>();
-        double sum_all = 0.0, sum_above = 0.0;
+        Sum sum_all, sum_above;
         unsigned n_above = 0;
         const float upper = few ? nextafterf(below_x, -CUDART_INF_F) : by_floor ? nextafterf(f32_from_ord(key_ord(floor)), -CUDART_INF_F) : above_x;
         each([&](const float (&v)[4], int i) {
@@ -597,10 +619,11 @@ struct Row {
             for (int e = 0; e < 4; ++e) {
                 const double whole = w[e] - kOne;
                 const bool over = k[e] && v[e] > upper;
-                if (k[e]) sum_all += whole;
-                if (over) sum_above += whole, ++n_above;
+                if (k[e]) sum_all.add(whole);
+                if (over) sum_above.add(whole), ++n_above;
                 in[e] = few ? over : k[e] && !over && v[e] >= below_x;
             }
+            sum_all.next(), sum_above.next();
             if (few) note(in, v, i);
             else if (in[0] | in[1] | in[2] | in[3]) {
 #pragma unroll
@@ -615,7 +638,7 @@ struct Row {
                     }
             }
         });
-        u64 w_all = warp_sum((u64)sum_all), w_above = warp_sum((u64)sum_above);
+        u64 w_all = warp_sum(sum_all.get()), w_above = warp_sum(sum_above.get());
         n_above = __reduce_add_sync(0xffffffffu, n_above);
         if (lane == 0) s.warp_w[warp] = w_all, s.above_w[warp] = w_above, s.above_n[warp] = n_above;
         __syncthreads();
@@ -827,15 +850,16 @@ struct Row {
     }
 };
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     extern __shared__ __align__(16) unsigned char s_raw[];
     SampleShared &s = *reinterpret_cast<SampleShared *>(s_raw);
     const long long row = blockIdx.x / a.ctas;
     const int rank = blockIdx.x % a.ctas;  // the cluster is the row's CTAs, in order
     const int start = min(rank * a.seg, a.vocab);
-    Row<T> w = {a, s, reinterpret_cast<T *>(s_raw + sizeof(SampleShared)), static_cast<const T *>(a.logits) + row * a.ld + start};
-    constexpr int PER = Row<T>::PER;
+    using R = Row<T, WIDE>;
+    R w = {a, s, reinterpret_cast<T *>(s_raw + sizeof(SampleShared)), static_cast<const T *>(a.logits) + row * a.ld + start};
+    constexpr int PER = R::PER;
     const int tid = w.tid = threadIdx.x, lane = w.lane = tid & 31, warp = w.warp = tid >> 5;
     w.rank = rank;
     w.start = start;
@@ -852,6 +876,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     s.octave[tid >> 3][tid & 7] = exp2((tid >> 3) / 128.0) * (double)(1ull << a.unit_bits);  // as many as threads
     if (a.ctas > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");  // waited for before the first write to another CTA
 
+    w.unit_bits = a.unit_bits;
     w.temp = temp;
     w.split = CUDART_INF_F;
     w.summed = false;
@@ -891,10 +916,25 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     unsigned top = __reduce_max_sync(0xffffffffu, own);
     if (lane == 0) s.warp_n[warp] = top;
     __syncthreads();
+    if constexpr (WIDE) {
+        // No entry weighs more than the largest that its thread has seen, so the weight of the CTA's entries is at most `each` times the
+        // sum of those.  In 2^-20, rounded up, with 1 % for the common factor of the weights and the roundings here.
+        top = __reduce_max_sync(0xffffffffu, s.warp_n[lane]);
+        const u64 each = (u64)(w.len / ST + PER + 1);  // entries of a thread, as they came in
+        u64 most = 0;
+        if (own > kNegInf) most = __float2ull_ru(w.lighter(largest, f32_from_ord(top)) * (1.01f * 1048576.0f)) + 1;
+        most = warp_sum(most) * each;
+        if (lane == 0) s.warp_w[warp] = most;
+        __syncthreads();
+    }
     if (a.ctas > 1) asm volatile("barrier.cluster.wait;" ::: "memory");  // every CTA of the cluster runs
     if (warp == 0) {
         top = __reduce_max_sync(0xffffffffu, s.warp_n[lane]);
         if (lane < a.ctas) s_put(s_at(&s.slot_top[rank], lane), top);
+        if constexpr (WIDE) {
+            const u64 most = warp_sum(s.warp_w[lane]);
+            if (lane < a.ctas) s_put(s_at(&s.slot_v[rank], lane), most);
+        }
     }
     w.sync();
     for (int r = 0; r < a.ctas; ++r) top = max(top, s.slot_top[r]);
@@ -914,6 +954,14 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     const double deep = 62.0 * 0.693147180559945309417232 * (double)temp;
     w.alone = !(w.top_wide - (double)nextafterf(w.top, -CUDART_INF_F) < deep);  // true for +infinity
     w.bottom = __double2float_rd(fmax(w.top_wide - deep, -(double)FLT_MAX));
+    if constexpr (WIDE) {
+        u64 most = 0;  // every CTA's bound, which is in weights of its own largest score, in the row's
+        if (lane < a.ctas) most = __float2ull_ru((float)s.slot_v[lane] * w.lighter(f32_from_ord(s.slot_top[lane]), w.top)) + 1;
+        most = warp_sum(most);
+        w.unit_bits = max(a.unit_bits, min(62 + 20 - (64 - __clzll((long long)most)), 49));
+        s.octave[tid >> 3][tid & 7] *= (double)(1ull << (w.unit_bits - a.unit_bits));
+        __syncthreads();
+    }
     w.floor = 0ull;
     if (least_in > 0.0f) {
         if (warp == 0) {
@@ -930,7 +978,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     u64 all = 0;
     if (k > 0 && k <= SLIST / 2) {
         w.template clear_bins<false>();
-        if (own > kNegInf) atomicAdd(&s.n[Row<T>::first_bin(w.distance(f32_from_ord(own)))], 1u);
+        if (own > kNegInf) atomicAdd(&s.n[R::first_bin(w.distance(f32_from_ord(own)))], 1u);
         w.template join_bins<false>();
         const int b = w.reach(s.all_n[tid], 0, (u64)k);
         if (b >= 0 && b < SBINS - 1) n = (int)w.gather_to(b);
@@ -964,7 +1012,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
         }, &count);
     count = __reduce_add_sync(0xffffffffu, count);
     if (lane == 0) s.warp_n[warp] = count;
-    w.template walk<true>(keep, Row<T>::aim(u, all));
+    w.template walk<true>(keep, R::aim(u, all));
     __syncthreads();
     if (s.found >= 0 && tid == 0) {
         a.ids[row] = start + s.found;
@@ -984,7 +1032,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     }
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 static int sample_launch(SampleArgs a, long long rows, int device, cudaStream_t st) {
     constexpr size_t kSmem = 227 * 1024;
     constexpr int kHold = (int)((kSmem - sizeof(SampleShared)) / sizeof(T)) & ~63;
@@ -998,13 +1046,13 @@ static int sample_launch(SampleArgs a, long long rows, int device, cudaStream_t 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     LK_TRY(asked.run(device, [&] {
-        LK_CUDA(cudaFuncSetAttribute((const void *)k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
-        LK_CUDA(cudaFuncSetAttribute((const void *)k_sample<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        LK_CUDA(cudaFuncSetAttribute((const void *)k_sample<T, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+        LK_CUDA(cudaFuncSetAttribute((const void *)k_sample<T, WIDE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         cfg.dynamicSmemBytes = kSmem;
         for (int c = 1; c <= SMAX_CTAS; ++c) {
             attr[0].val.clusterDim.x = (unsigned)c;
             cfg.gridDim = dim3((unsigned)c);
-            if (cudaOccupancyMaxActiveClusters(&fit[device][c], k_sample<T>, &cfg) != cudaSuccess) fit[device][c] = 0;
+            if (cudaOccupancyMaxActiveClusters(&fit[device][c], k_sample<T, WIDE>, &cfg) != cudaSuccess) fit[device][c] = 0;
         }
         cudaGetLastError();
         return 0;
@@ -1026,7 +1074,7 @@ static int sample_launch(SampleArgs a, long long rows, int device, cudaStream_t 
     cfg.gridDim = dim3((unsigned)(rows * a.ctas));
     cfg.dynamicSmemBytes = sizeof(SampleShared) + (size_t)a.cap * sizeof(T);
     cfg.stream = st;
-    return launch_cfg("lk_sample", k_sample<T>, cfg, a);
+    return launch_cfg("lk_sample", k_sample<T, WIDE>, cfg, a);
 }
 
 }  // namespace lk
@@ -1054,7 +1102,8 @@ extern "C" int lk_sample(int device, int dtype, int64_t rows, int64_t vocab, con
     SampleArgs a = {d_logits, ld, (int)vocab, 1, 0, 0, d_temperature, d_top_p, d_min_p, d_u, d_top_k,
                     reinterpret_cast<long long *>(d_ids), d_probs, d_kept, std::min(62 - bits, 49)};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == LK_F32) return sample_launch<float>(a, rows, device, st);
-    if (dtype == LK_F16) return sample_launch<__half>(a, rows, device, st);
-    return sample_launch<__nv_bfloat16>(a, rows, device, st);
+    const bool wide = vocab > kWide;
+    if (dtype == LK_F32) return wide ? sample_launch<float, true>(a, rows, device, st) : sample_launch<float, false>(a, rows, device, st);
+    if (dtype == LK_F16) return wide ? sample_launch<__half, true>(a, rows, device, st) : sample_launch<__half, false>(a, rows, device, st);
+    return wide ? sample_launch<__nv_bfloat16, true>(a, rows, device, st) : sample_launch<__nv_bfloat16, false>(a, rows, device, st);
 }
