@@ -14,8 +14,24 @@ struct LinearArgs {
     int act, out_type;
 };
 
-// The activation of N values: one branch for all of them.
-template <int N>
+// The share of a normal distribution beyond a, 0 <= a <= 20: exp(-a^2 / 2) P(t), t = 1 / (1 + 0.295 a), with P fitted (weighted least
+// squares after Lawson) to exp(a^2 / 2) erfc(a / sqrt 2) / 2, 4e-8 relative.  1 + erf, which is twice this, cancels below 0.
+// FULL: within 14 * 2^-24 relative, with t corrected (to 2^-24; P is 2.7 times as sensitive to it) and what a^2 lost brought back in.
+// Else those two are left out, 2^-24 * (27 + 4 a^2 / 2).  With erfcf in its place 4,096 x 8,192 x 1,024 bf16 took 130 us instead of 90.
+template <bool FULL>
+__device__ __forceinline__ float normal_tail(float a) {
+    const float d = fmaf(0.295f, a, 1.0f), h = a * a;
+    float t = __fdividef(1.0f, d);
+    if (FULL) t = fmaf(t, fmaf(-fmaf(0.295f, a, 1.0f - d), t, fmaf(-d, t, 1.0f)), t);
+    float p = 0.0392500758f;
+    p = fmaf(p, t, -0.182633162f), p = fmaf(p, t, 0.269538283f), p = fmaf(p, t, -0.11551214f), p = fmaf(p, t, 0.165299833f);
+    p = fmaf(p, t, 0.0851306245f), p = fmaf(p, t, 0.121609196f), p = fmaf(p, t, 0.117300875f), p = fmaf(p, t, 1.6388547e-05f);
+    if (FULL) return p * expf(-0.5f * h) * fmaf(-0.5f, fmaf(a, a, -h), 1.0f);  // the last: what h lost
+    return p * __expf(-0.5f * h);
+}
+
+// The activation of N values: one branch for all of them.  FULL for float32 results; 16-bit ones hold fewer bits than what is saved.
+template <bool FULL, int N>
 __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
     if (act == LK_ACT_RELU) {
 #pragma unroll
@@ -25,7 +41,10 @@ __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
         for (int u = 0; u < N; ++u) v[u] = __fdividef(v[u], 1.0f + __expf(-v[u]));
     } else if (act == LK_ACT_GELU) {
 #pragma unroll
-        for (int u = 0; u < N; ++u) v[u] = 0.5f * v[u] * (1.0f + erff(v[u] * 0.70710678118654752f));
+        for (int u = 0; u < N; ++u) {
+            const float q = normal_tail<FULL>(fminf(fabsf(v[u]), 20.0f));
+            v[u] *= v[u] < 0.0f ? q : 1.0f - q;
+        }
     } else if (act == LK_ACT_GELU_TANH) {
         // (1 + tanh z) / 2 = 1 / (1 + exp(-2 z))
 #pragma unroll
@@ -49,7 +68,8 @@ __device__ __forceinline__ void finish_one(const LinearArgs &p, long long i, lon
     float v = acc * (scale_of(p.a_scales, i) * scale_of(p.w_scales, j));
     if (p.bias != nullptr) v += load_as(p.out_type, p.bias, j);
     float y[1] = {v};
-    activate_all<1>(p.act, y);
+    if (p.out_type == LK_F32) activate_all<true>(p.act, y);
+    else activate_all<false>(p.act, y);
     if (p.residual != nullptr) y[0] += load_as(p.out_type, p.residual, i * p.ldr + j);
     store_as(p.out_type, p.out, i * p.ldo + j, y[0]);
 }

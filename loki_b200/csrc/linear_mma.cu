@@ -21,6 +21,7 @@
 //
 // Every wait is bounded; a CTA that gives up raises g_linear_failed, which lk_ops_status reports.
 #include <cstddef>
+#include <type_traits>
 
 #include "linear.cuh"
 #include "tensor5.cuh"
@@ -356,7 +357,7 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
 #pragma unroll
                     for (int u = 0; u < LCHUNK; ++u) x[u] = fmaf(l_sum<I8>(v[u]), sw, bias);
                 }
-                activate_all<LCHUNK>(p.act, x);
+                activate_all<std::is_same<Out, float>::value>(p.act, x);
                 if (p.residual != nullptr) {
 #pragma unroll
                     for (int u = 0; u < LCHUNK; ++u) x[u] += rx[u];
@@ -422,7 +423,7 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) x[u] = fmaf(I8 ? (float)whole[u] : x[u], sa[u] * sw, bias);
-            activate_all<4>(p.act, x);
+            activate_all<std::is_same<Out, float>::value>(p.act, x);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (live && u < w && i + u < p.m)
