@@ -364,7 +364,9 @@ LK_API int lk_rms_norm_i8(int device, int dtype, int64_t rows, int dim, const vo
 
 /* Matrix product of rows with rows, with its epilogue:
  *   out[i, j] = act(scale_a[i] * scale_w[j] * sum_l a[i, l] * w[j, l] + bias[j]) + residual[i, j]
- * rounded once, to out_dtype.  For LK_I8 the sum is the exact int32 dot (as in lk_search); for
+ * rounded once, to out_dtype (a float32 result's activation is within 15 * 2^-24 of its input's, relative,
+ * 2^-24 * (7 |t| + 12) with t = 2 sqrt(2 / pi) (v + 0.044715 v^3) for the tanh form; a 16-bit one's within
+ * 2^-24 * (27 + 2 v^2), 2^-24 * (8 + 8 |t|) with t = v for SiLU, before it is rounded).  For LK_I8 the sum is the exact int32 dot (as in lk_search); for
  * LK_F16 / LK_BF16 products are exact and accumulated in float32.
  *   dtype       LK_I8, LK_F16 or LK_BF16: type of a (m x k) and w (n x k)
  *   k           at most LK_LINEAR_MAX_K; k = 0 gives act(bias) + residual

@@ -30,6 +30,15 @@ __device__ __forceinline__ float normal_tail(float a) {
     return p * __expf(-0.5f * h);
 }
 
+// v / (1 + exp(-t)), t of v's sign.  FULL: to 12 * 2^-24, also where the exponential of -t would pass float32's range (v < -88 of SiLU); else
+// with the fast exponential and quotient, 2^-24 * 8 (1 + |t|).
+template <bool FULL>
+__device__ __forceinline__ float gated(float v, float t) {
+    if (!FULL) return __fdividef(v, 1.0f + __expf(-t));
+    const float e = expf(-fabsf(t));
+    return __fdividef(t < 0.0f ? v * e : v, 1.0f + e);  // 2 ulp; a division rounded to half of one took 20 % longer over a small product
+}
+
 // The activation of N values: one branch for all of them.  FULL for float32 results; 16-bit ones hold fewer bits than what is saved.
 template <bool FULL, int N>
 __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
@@ -38,7 +47,7 @@ __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
         for (int u = 0; u < N; ++u) v[u] = v[u] < 0.0f ? 0.0f : v[u];  // NaN stays
     } else if (act == LK_ACT_SILU) {
 #pragma unroll
-        for (int u = 0; u < N; ++u) v[u] = __fdividef(v[u], 1.0f + __expf(-v[u]));
+        for (int u = 0; u < N; ++u) v[u] = gated<FULL>(v[u], v[u]);
     } else if (act == LK_ACT_GELU) {
 #pragma unroll
         for (int u = 0; u < N; ++u) {
@@ -50,7 +59,7 @@ __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const float z = 0.79788456080286536f * (v[u] + 0.044715f * v[u] * v[u] * v[u]);
-            v[u] = __fdividef(v[u], 1.0f + __expf(-2.0f * z));
+            v[u] = gated<FULL>(v[u], 2.0f * z);
         }
     }
 }

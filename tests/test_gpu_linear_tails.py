@@ -2,7 +2,8 @@
 
 The product is of zeros and the value comes from the bias, so an activation's input is exact.  Bounds for float32 results, with
 e = 2^-24 (half a step), CUDA's stated 2 ulp (4 e) for expf and __fdividef:
-SiLU v / (1 + exp(-v)): the exponential 4 e, a product, a sum and a quotient e each (of the sum's 4 e at most what the exponential has): 12 e.
+SiLU v / (1 + exp(-v)), below 0 v exp(v) / (1 + exp(v)): the exponential 4 e and, halved, again in the sum; a product and the sum e each, the
+quotient 4 e: 12 e.
 GELU v Phi(v): below 0 Phi is exp(-v^2 / 2) P(t) with t = 1 / (1 + c |v|) to e, to which P is 2.71 times as sensitive; the fit 0.7 e, P's
 additions 3 e, the exponential 4 e, products 4 e: 15 e.  Above 0 it is 1 minus such a tail.
 GELU (tanh) v / (1 + exp(-t)), t = 2 sqrt(2 / pi) (v + 0.044715 v^3): t carries 7 e (its constants and products), so 7 |t| + 12.
@@ -49,7 +50,7 @@ REACH = {"silu": 80.0, "gelu": 12.5, "gelu_tanh": 9.0}
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("act", ["gelu"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("m,aligned", [(1, True), (40, True), (300, True), (3, False)])
 def test_relative_to_the_result(ops, act, out, m, aligned):
     n, k = 4096, 64
@@ -69,7 +70,7 @@ def test_relative_to_the_result(ops, act, out, m, aligned):
     assert not bad.any(), (v[np.nonzero(bad)[1][:4]], got[bad][:4], want[np.nonzero(bad)[1][:4]], (np.abs(got - want) / np.maximum(off, 1e-300)).max())
 
 
-@pytest.mark.parametrize("act", ["gelu"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
 def test_the_ends(ops, act):
     """Far out the results are 0 and the value itself, down to the type's lowest and up to its largest; NaN stays NaN."""
     big = torch.finfo(torch.bfloat16).max  # a float32 as well
