@@ -8,7 +8,8 @@ They are the functions ``lk_rms_norm_i8``, ``lk_linear`` and ``lk_sample`` of ``
 which states the formulas; here the arguments are PyTorch tensors.  A call runs on the device of its
 first tensor, on PyTorch's current stream of that device, returns without waiting and can be captured
 into a CUDA graph.  Tensors are two-dimensional with contiguous rows (``stride(1) == 1``) at any row
-stride; vectors are contiguous.  There is no gradient: a tensor that requires one is refused.
+stride; vectors are contiguous.  There is no gradient: a tensor that requires one, or carries a
+forward-mode derivative, is refused.
 
     codes, scales, hidden = ops.rms_norm_i8(x, gain, residual=hidden)
     scores = ops.linear(codes, table, a_scales=scales, w_scales=table_scales, out_dtype=torch.float32)
@@ -17,6 +18,7 @@ stride; vectors are contiguous.  There is no gradient: a tensor that requires on
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as _forward
 
 from . import _lib
 from ._lib import LK_EDIM, LK_EINVAL, LokiError, check, lib
@@ -46,6 +48,8 @@ def _why(t, what, types, index, *shape):
         _refuse(LK_EINVAL, f"{what}: its rows are not contiguous")
     if t.requires_grad and torch.is_grad_enabled():
         _refuse(LK_EINVAL, f"{what}: it requires a gradient, which this operator does not have")
+    if _forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None:
+        _refuse(LK_EINVAL, f"{what}: it carries a forward-mode derivative, which this operator does not have")
     _refuse(LK_EINVAL, f"{what}: its rows overlap")
 
 
@@ -59,7 +63,8 @@ def _matrix(t, what, types, index=None, rows=None, cols=None):
     except (AttributeError, ValueError):
         _why(t, what, types, index, rows, cols)
     if (on < 0 or t.dtype not in types or (one != 1 and c > 1) or (index is not None and on != index) or (rows is not None and r != rows)
-            or (cols is not None and c != cols) or (ld < c and r > 1) or (t.requires_grad and torch.is_grad_enabled())):
+            or (cols is not None and c != cols) or (ld < c and r > 1) or (t.requires_grad and torch.is_grad_enabled())
+            or (_forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None)):
         _why(t, what, types, index, rows, cols)
     return r, c, ld if r > 1 else max(ld, c), on  # a single row's stride says nothing
 
@@ -70,7 +75,8 @@ def _vector(t, what, types, index, n):
         return None
     try:
         if (t.get_device() != index or t.dtype not in types or t.shape != (n,) or (n > 1 and t.stride() != (1,))
-                or (t.requires_grad and torch.is_grad_enabled())):
+                or (t.requires_grad and torch.is_grad_enabled())
+                or (_forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None)):
             _why(t, what, types, index, n)
     except AttributeError:
         _why(t, what, types, index, n)

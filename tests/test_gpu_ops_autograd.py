@@ -1,0 +1,54 @@
+"""GPU: what the operators say to autograd: a tensor that carries a derivative is refused."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(lk):
+    from loki_b200 import ops
+    return ops
+
+
+def calls(ops):
+    """name -> (function of one floating tensor, that tensor)"""
+    x, gain, u = torch.randn(4, 64, device="cuda"), torch.rand(64, device="cuda"), torch.rand(4, device="cuda")
+    h, w = x.half(), torch.randn(8, 64, device="cuda").half()
+    codes = torch.ones(4, 64, dtype=torch.int8, device="cuda")
+    table = torch.ones(8, 64, dtype=torch.int8, device="cuda")
+    return {
+        "x": (lambda t: ops.rms_norm_i8(t, gain), x), "gain": (lambda t: ops.rms_norm_i8(x, t), gain),
+        "norm residual": (lambda t: ops.rms_norm_i8(x, gain, residual=t), x),
+        "a": (lambda t: ops.linear(t, w), h), "w": (lambda t: ops.linear(h, t), w),
+        "a_scales": (lambda t: ops.linear(codes, table, a_scales=t), u), "bias": (lambda t: ops.linear(h, w, bias=t), w[:, 0].contiguous()),
+        "residual": (lambda t: ops.linear(h, w, residual=t), torch.ones(4, 8, device="cuda").half()),
+        "scores": (lambda t: ops.sample(t, u), x), "u": (lambda t: ops.sample(x, t), u), "temperature": (lambda t: ops.sample(x, u, temperature=t), u),
+        "top_p": (lambda t: ops.sample(x, u, top_p=t), u), "min_p": (lambda t: ops.sample(x, u, min_p=t), u),
+    }
+
+
+NAMES = ["x", "gain", "norm residual", "a", "w", "a_scales", "bias", "residual", "scores", "u", "temperature", "top_p", "min_p"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_dual_tensors_are_refused(ops, lk, name):
+    call, t = calls(ops)[name]
+    with fwd.dual_level():
+        with pytest.raises(lk.LokiError, match="derivative"):
+            call(fwd.make_dual(t, torch.ones_like(t)))
+        call(t)  # one without a tangent is an ordinary tensor
+    call(t)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_transformed_tensors_are_refused(ops, lk, name):
+    call, t = calls(ops)[name]
+    first = lambda v: call(v)[0]
+    with pytest.raises((lk.LokiError, RuntimeError)):
+        torch.func.jvp(first, (t,), (torch.ones_like(t),))
+    with pytest.raises((lk.LokiError, RuntimeError)):
+        torch.func.vmap(first)(t.expand(2, *t.shape))
+    with pytest.raises((lk.LokiError, RuntimeError)):
+        torch.func.grad(lambda v: first(v).float().sum())(t)
