@@ -89,6 +89,7 @@ _F32, _I32, _I64, _I8 = (torch.float32,), (torch.int32,), (torch.int64,), (torch
 
 
 _new = torch.empty_strided
+_written = torch.autograd.graph.increment_version  # for tensors that the caller gives: autograd does not see the kernels' writes
 
 
 def rms_norm_i8(x, gain=None, *, residual=None, eps: float = 1e-6, out_codes=None, out_scales=None, out_sum=None):
@@ -108,13 +109,16 @@ def rms_norm_i8(x, gain=None, *, residual=None, eps: float = 1e-6, out_codes=Non
         r = residual.data_ptr()
     place = x.device
     s = lds = 0
+    given = ()
     if out_sum is not None:
+        given = (out_sum,)
         lds = _matrix(out_sum, "out_sum", (kind,), dev, rows, dim)[2]
         s = out_sum.data_ptr()
     elif residual is not None:
         out_sum, lds = _new((rows, dim), (dim, 1), dtype=kind, device=place), dim
         s = out_sum.data_ptr()
     if out_codes is not None:
+        given += (out_codes,)
         ldc = _matrix(out_codes, "out_codes", _I8, dev, rows, dim)[2]
     else:  # rows on 16-byte boundaries, as linear reads them best
         ldc = (dim + 15) // 16 * 16
@@ -123,11 +127,14 @@ def rms_norm_i8(x, gain=None, *, residual=None, eps: float = 1e-6, out_codes=Non
         out_scales = _new((rows,), (1,), dtype=torch.float32, device=place)
         scales = out_scales.data_ptr()
     else:
+        given += (out_scales,)
         scales = _vector(out_scales, "out_scales", _F32, dev, rows)
     st = _norm(dev, _FLOATS[kind], rows, dim, x.data_ptr(), ldx, r, ldr, g, 0 if g is None else _FLOATS[gain.dtype], eps,
                             s, lds, out_codes.data_ptr(), ldc, scales, _stream(dev))
     if st:
         check(st)
+    if given:
+        _written(given)
     return out_codes, out_scales, out_sum
 
 
@@ -170,7 +177,8 @@ def linear(a, w, *, a_scales=None, w_scales=None, bias=None, act: str = "none", 
     sa = None if a_scales is None else _vector(a_scales, "a_scales", _F32, dev, m)
     sw = None if w_scales is None else _vector(w_scales, "w_scales", _F32, dev, n)
     b = None if bias is None else _vector(bias, "bias", (kind,), dev, n)
-    if out is None:
+    given = out is not None
+    if not given:
         out, ldo = _new((m, n), (n, 1), dtype=kind, device=a.device), n
     else:
         ldo = _matrix(out, "out", (kind,), dev, m, n)[2]
@@ -178,6 +186,8 @@ def linear(a, w, *, a_scales=None, w_scales=None, bias=None, act: str = "none", 
                  result, out.data_ptr(), ldo, _stream(dev))
     if st:
         check(st)
+    if given:
+        _written(out)
     return out
 
 
@@ -217,4 +227,6 @@ def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, o
                        _vector(ids, "out_ids", _I64, dev, rows), probs.data_ptr(), kept.data_ptr(), _stream(dev))
     if st:
         check(st)
+    if out_ids is not None:
+        _written(out_ids)
     return ids, probs, kept

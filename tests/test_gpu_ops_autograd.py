@@ -1,4 +1,4 @@
-"""GPU: what the operators say to autograd: a tensor that carries a derivative is refused."""
+"""GPU: what the operators say to autograd: a tensor that carries a derivative is refused, one that is written is marked as written."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -52,3 +52,28 @@ def test_transformed_tensors_are_refused(ops, lk, name):
         torch.func.vmap(first)(t.expand(2, *t.shape))
     with pytest.raises((lk.LokiError, RuntimeError)):
         torch.func.grad(lambda v: first(v).float().sum())(t)
+
+
+def test_results_in_given_tensors_are_writes(ops):
+    x, u = torch.randn(4, 64, device="cuda"), torch.rand(4, device="cuda")
+    h, w = x.half(), torch.randn(8, 64, device="cuda").half()
+    outs = {
+        "out": (lambda t: ops.linear(h, w, out=t), torch.zeros(4, 8, device="cuda").half()),
+        "out_sum": (lambda t: ops.rms_norm_i8(x, residual=x, out_sum=t), torch.zeros(4, 64, device="cuda")),
+        "in place": (lambda t: ops.rms_norm_i8(x, residual=t, out_sum=t), torch.zeros(4, 64, device="cuda")),
+        "out_codes": (lambda t: ops.rms_norm_i8(x, out_codes=t), torch.zeros(4, 64, dtype=torch.int8, device="cuda")),
+        "out_scales": (lambda t: ops.rms_norm_i8(x, out_scales=t), torch.zeros(4, device="cuda")),
+        "out_ids": (lambda t: ops.sample(x, u, out_ids=t), torch.zeros(4, dtype=torch.int64, device="cuda")),
+    }
+    for name, (call, t) in outs.items():
+        before = t._version
+        call(t)
+        assert t._version > before, name
+        with torch.inference_mode():  # tensors that keep no count
+            call(t.clone())
+    leaf = torch.ones(4, 8, device="cuda", requires_grad=True)
+    saved = torch.zeros(4, 8, device="cuda")
+    y = (leaf * saved).sum()
+    ops.linear(h, w, out=saved, out_dtype=torch.float32)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
