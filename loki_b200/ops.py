@@ -192,8 +192,16 @@ def linear(a, w, *, a_scales=None, w_scales=None, bias=None, act: str = "none", 
 
 
 def check_device(device=0):
-    """Wait for the device; raise if a bounded wait inside one of these kernels ran out since the last call."""
-    index = torch.device("cuda", device).index if isinstance(device, int) else torch.device(device).index
+    """Wait for the device (a number, a name or a ``torch.device``; the current one for ``"cuda"`` or None); raise if a
+    bounded wait inside one of these kernels ran out since the last call."""
+    index = device
+    if not isinstance(device, int):
+        named = torch.device("cuda" if device is None else device)
+        if named.type != "cuda":
+            _refuse(LK_EINVAL, f"device: a CUDA device is wanted, not {named}")
+        index = named.index
+        if index is None:
+            index = torch.cuda.current_device() if torch.cuda.is_available() else 0
     check(lib.lk_ops_status(index))
 
 
