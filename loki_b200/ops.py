@@ -17,11 +17,14 @@ forward-mode derivative, is refused.
 """
 from __future__ import annotations
 
+import math
+import numbers
+
 import torch
 import torch.autograd.forward_ad as _forward
 
 from . import _lib
-from ._lib import LK_EDIM, LK_EINVAL, LokiError, check, lib
+from ._lib import LK_EDIM, LK_EINVAL, LK_ERANGE, LokiError, check, lib
 
 _FLOATS = {torch.float32: _lib.LK_F32, torch.float16: _lib.LK_F16, torch.bfloat16: _lib.LK_BF16}
 _OPERANDS = {torch.int8: _lib.LK_I8, torch.float16: _lib.LK_F16, torch.bfloat16: _lib.LK_BF16}
@@ -85,6 +88,7 @@ def _vector(t, what, types, index, n):
 
 _stream = torch._C._cuda_getCurrentRawStream
 _norm, _linear, _sample = lib.lk_rms_norm_i8, lib.lk_linear, lib.lk_sample
+_F32_MAX = torch.finfo(torch.float32).max
 _F32, _I32, _I64, _I8 = (torch.float32,), (torch.int32,), (torch.int64,), (torch.int8,)
 
 
@@ -205,10 +209,25 @@ def check_device(device=0):
     check(lib.lk_ops_status(index))
 
 
+def _number(v, what, types):
+    """A number for all rows, as the type of the vectors can hold it."""
+    if not isinstance(v, numbers.Real):
+        _refuse(LK_EINVAL, f"{what}: a CUDA tensor or a number is wanted")
+    if types is _I32:
+        if not isinstance(v, numbers.Integral) and not (math.isfinite(v) and v == int(v)):
+            _refuse(LK_EINVAL, f"{what}: {v} is not a whole number")
+        if not -(1 << 31) <= v < 1 << 31:
+            _refuse(LK_ERANGE, f"{what}: {v} is outside int32")
+        return int(v)
+    if _F32_MAX < abs(v) < math.inf:
+        _refuse(LK_ERANGE, f"{what}: {v} is outside float32")
+    return float(v)
+
+
 def _per_row(v, what, types, scores, rows, dev):
     """(address, tensor) of one value per row: a vector, or a number for all rows."""
     if v is not None and not isinstance(v, torch.Tensor):
-        v = scores.new_full((rows,), v, dtype=types[0])
+        v = scores.new_full((rows,), _number(v, what, types), dtype=types[0])
     return _vector(v, what, types, dev, rows), v
 
 
@@ -217,7 +236,7 @@ def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, o
     -> (ids [rows] int64, probs [rows] float32, kept [rows] int32).
 
     ``temperature``, ``top_p``, ``min_p`` (float32) and ``top_k`` (int32) are vectors of one value per row, or
-    numbers for all rows; None switches a filter off.  ``probs`` is the probability of the draw among the
+    numbers for all rows (``top_k`` a whole one); None switches a filter off.  ``probs`` is the probability of the draw among the
     ``kept`` entries.  A row with nothing to draw (only NaN and -inf) gets id -1.
     """
     rows, vocab, ld, dev = _matrix(scores, "scores", _FLOATS)
