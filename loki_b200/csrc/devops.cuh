@@ -34,33 +34,6 @@ struct Elem<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
 };
 
-// Eight consecutive elements at a 16-byte boundary, as float32.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-        const uint4 a = *reinterpret_cast<const uint4 *>(p);
-        const T *e = reinterpret_cast<const T *>(&a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = Elem<T>::get(e[i]);
-    }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        uint4 a;
-        T *e = reinterpret_cast<T *>(&a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = Elem<T>::put(v[i]);
-        *reinterpret_cast<uint4 *>(p) = a;
-    }
-}
-
 // One value of a type known at run time (LK_F32 / LK_F16 / LK_BF16).
 __device__ __forceinline__ float load_as(int dtype, const void *p, long long i) {
     if (dtype == LK_F32) return static_cast<const float *>(p)[i];
