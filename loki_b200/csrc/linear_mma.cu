@@ -435,6 +435,12 @@ k_linear_mma(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ C
     if (joined && warp < 2) asm volatile("barrier.cluster.wait;" ::: "memory");
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (joined && ctl->failed != 0) {
+        // This CTA did not wait for the others' parts, and one of them may still be on its way to sending its own here.  The barrier opens
+        // when the other CTAs' threads have come here too or, as those that did not fail, have exited; all their waits are bounded.
+        asm volatile("barrier.cluster.arrive;" ::: "memory");
+        asm volatile("barrier.cluster.wait;" ::: "memory");
+    }
     if (tid == 0 && ctl->failed != 0) {
         atomicExch(&g_linear_failed, 1u);
         // copies this CTA issued may still be landing in its shared memory: give them time before it is released
