@@ -33,7 +33,9 @@ constexpr int LSLICE = 128;         // bytes of K per stage: one swizzle row
 constexpr int LW_BYTES = LW * LSLICE;
 constexpr int LEPI_WARPS = 16;      // four per tensor-memory quadrant, 16 columns of a tile at a time each
 constexpr int LTHREADS = 64 + LEPI_WARPS * 32;
-constexpr int LMAX_STAGES = 8;        // 8,192 x 18 KB slices of an m = 8 product: 26.4 us with 8 stages, 27.6 with 6, 28.4 with 12
+// A long stream, 8,192 x 18 KB slices of an m = 8 product: 26.4 us with 8 stages, 27.6 with 6, 28.4 with 12.  Nothing else was measured: for one
+// tile of few slices more would fit (11 with 32 rows of a), and the latency that linear_plan counts per stage is paid twice there.
+constexpr int LMAX_STAGES = 8;
 constexpr int LCHUNK = 16;          // columns an epilogue thread holds at a time
 
 static __device__ unsigned g_linear_failed;  // a bounded wait ran out on this device
@@ -52,7 +54,7 @@ struct LinearTiles {
 // Place of tile t: bands of `band` tiles of w's rows, through which the tiles of a's rows run.  Where w is the smaller operand a
 // band as wide as w keeps it in L2 and reads a once: 8,192 x 4,096 x 4,096 bf16, sustained: 228 us with bands of 1, 216 of 8, 208 of
 // all 16.  Else bands of 8, which also serve an `a` that is too large to stay (4,096 x 8,192 x 4,096 int8: 102.5 us with bands of 1,
-// 103.7 of 8, 105.5 of 16).
+// 103.7 of 8, 105.5 of 16).  These two sizes are all that was timed.
 __device__ __forceinline__ void tile_at(const LinearTiles &g, long long t, int &tn, int &tm) {
     const long long per = (long long)g.band * g.tiles_m;
     const int band = (int)(t / per), r = (int)(t - band * per);
@@ -506,7 +508,8 @@ static int ring_stages(int mt, int cg, int split) {
 }
 
 // The tile that finishes first, by an account of one CTA's clocks whose constants were fitted to 110 shapes (m 1 to 1,024,
-// five n x k, int8 and bf16) with every tile timed; over them the choice costs 0.2 % against the best tile, 4 % at worst.
+// five n x k, int8 and bf16) with every tile timed; over them the choice costs 0.2 % against the best tile, 4 % at worst.  Outside them
+// (m to 8,192, k to 65,536) it is an extrapolation.
 // A slice of K: its MMAs (0.62 clocks per row of a), its bytes at 58 per clock and SM and 5,456 for all CTAs together, and the
 // 4,058 clocks from asking for a slice to having it, shared by the stages.  A tile's epilogue, 31 clocks per row of a, runs under
 // the next tile's slices; the last one shows.  Joining parts of K costs 4,305 clocks and 16 per row of a.

@@ -60,7 +60,8 @@ constexpr int SD_SHIFT = 16, SD_BASE = (127 - 3) << 7;  // bins by d: exponent a
 using u64 = unsigned long long;
 // Measured with a top-p alone, 1 to 512 rows of 4,096 to 1,000,000 scores: a CTA's time per entry over all passes, and for one that
 // its shared memory does not hold, its start and its sorts, and what the meetings of a cluster add, and of one of more
-// than eight.  A row with a small top-k costs less per entry, but the host does not see the filters.
+// than eight.  A row with a small top-k costs less per entry, but the host does not see the filters.  Over 92 shapes and filters the
+// number of CTAs that follows costs 1.3 % against the best uniform number on average, 25 % at worst (100 rows of 151,936, mixed filters).
 constexpr double SAMPLE_ENTRY_NS = 0.5, SAMPLE_AWAY_NS = 0.15, SAMPLE_CTA_NS = 15000.0, SAMPLE_MEET_NS = 8000.0, SAMPLE_WIDE_NS = 6000.0;
 
 struct alignas(16) SampleShared {

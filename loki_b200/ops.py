@@ -236,7 +236,7 @@ def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, o
     -> (ids [rows] int64, probs [rows] float32, kept [rows] int32).
 
     ``temperature``, ``top_p``, ``min_p`` (float32) and ``top_k`` (int32) are vectors of one value per row, or
-    numbers for all rows (``top_k`` a whole one); None switches a filter off.  ``probs`` is the probability of the draw among the
+    numbers for all rows (``top_k`` a whole one; a number costs a kernel that fills a vector); None switches a filter off.  ``probs`` is the probability of the draw among the
     ``kept`` entries.  A row with nothing to draw (only NaN and -inf) gets id -1.
     """
     rows, vocab, ld, dev = _matrix(scores, "scores", _FLOATS)
