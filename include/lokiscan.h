@@ -408,7 +408,7 @@ LK_API int lk_ops_status(int device);
  *   d_temperature  rows floats, NULL = 1 everywhere; 0 = the largest score (top_k = 1)
  *   d_top_k        rows int32, NULL or <= 0 = all
  *   d_top_p        rows floats, NULL or >= 1 = all; <= 0 = only the first
- *   d_min_p        rows floats, NULL or <= 0 = all
+ *   d_min_p        rows floats, NULL or <= 0 = all; above 1 = 1 (what weighs as much as the first)
  *   d_u            rows floats in [0, 1); others are taken as the nearest number of that range
  *   d_ids          rows int64;  d_probs (may be NULL) the weight of the draw over the kept weight;
  *                  d_kept (may be NULL) how many were kept

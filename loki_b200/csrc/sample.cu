@@ -984,7 +984,7 @@ __global__ void __launch_bounds__(ST) k_sample(const SampleArgs a) {
     w.floor = 0ull;
     if (least_in > 0.0f) {
         if (warp == 0) {
-            const u64 f = w.lowest(least_in);
+            const u64 f = w.lowest(fminf(least_in, 1.0f));
             if (lane == 0) s.floor = f;
         }
         __syncthreads();
